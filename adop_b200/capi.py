@@ -13,6 +13,9 @@ MAX_CHANNELS = 32
 ADOP_OK = 0
 CAMERA_PINHOLE_DISTORTION = 0
 CAMERA_OCAM = 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_ELU, ACTIVATION_SILU = 0, 1, 2, 3
+NORM_MAX_CHANNELS = 4096
 
 _c_float_p = C.c_void_p  # all data pointers travel as raw addresses
 
@@ -77,6 +80,21 @@ class AdopTonemapGrads(C.Structure):
                 ("accumulate", C.c_int32)]
 
 
+class AdopNormImage(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("image_stride", C.c_int64), ("pixel_stride", C.c_int64)]
+
+
+class AdopNormParams(C.Structure):
+    _fields_ = [("batch", C.c_int32), ("channels", C.c_int32), ("pixels", C.c_int64), ("num_groups", C.c_int32), ("type", C.c_int32),
+                ("param_type", C.c_int32), ("activation", C.c_int32), ("eps", C.c_float), ("weight", C.c_void_p), ("bias", C.c_void_p)]
+
+
+class AdopNormIO(C.Structure):
+    _fields_ = [("x", AdopNormImage), ("gate", AdopNormImage), ("y", AdopNormImage), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+                ("grad_y", AdopNormImage), ("grad_x", AdopNormImage), ("grad_gate", AdopNormImage), ("grad_weight", C.c_void_p),
+                ("grad_bias", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 class AdopPeerHandle(C.Structure):
     _fields_ = [("bytes", C.c_ubyte * 64)]
 
@@ -125,6 +143,8 @@ EXPORTED_SYMBOLS = [
     "adop_points_morton_workspace_bytes", "adop_points_morton_order", "adop_points_permute",
     "adop_points_block_shuffle_order", "adop_points_sort_blocks_by_radius_order",
     "adop_points_knn_workspace_bytes", "adop_points_knn_distance", "adop_points_radius_sample",
+    "adop_group_norm_workspace_bytes", "adop_group_norm_forward", "adop_group_norm_backward",
+    "adop_gated_activation_forward", "adop_gated_activation_backward",
 ]
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -208,6 +228,11 @@ def load_library():
     lib.adop_points_radius_sample.restype = C.c_int
     lib.adop_points_permute.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]
     lib.adop_points_permute.restype = C.c_int
+    lib.adop_group_norm_workspace_bytes.argtypes = [C.POINTER(AdopNormParams), C.c_int32, C.c_int32]
+    lib.adop_group_norm_workspace_bytes.restype = C.c_size_t
+    for name in ("adop_group_norm_forward", "adop_group_norm_backward", "adop_gated_activation_forward", "adop_gated_activation_backward"):
+        getattr(lib, name).argtypes = [C.POINTER(AdopNormParams), C.POINTER(AdopNormIO), C.c_void_p]
+        getattr(lib, name).restype = C.c_int
     lib.adop_profile_enable.argtypes = [C.c_int32]
     lib.adop_profile_enable.restype = C.c_int
     lib.adop_profile_collect.argtypes = [C.POINTER(AdopKernelTime), C.c_int32]

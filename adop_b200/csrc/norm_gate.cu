@@ -1,0 +1,388 @@
+// Host side of the group normalisation with an activation and of the gate of a gated convolution: argument checks, which
+// kernel and launch shape a call takes, and the C ABI. The kernels are in norm_gate.cuh, compiled once per image type.
+#include "common.cuh"
+#include "norm_gate.h"
+#include "per_device.h"
+
+namespace adop {
+
+namespace {
+
+int64_t gcd64(int64_t a, int64_t b)
+{
+    while (b) { const int64_t r = a % b; a = b; b = r; }
+    return a;
+}
+
+adop_status refuse(adop_status s, const char* why)
+{
+    snprintf(last_error_buffer(), 512, "%s", why);
+    return s;
+}
+
+int element_size(int type) { return type == ADOP_TYPE_F32 ? 4 : 2; }
+
+adop_status check_params(const adop_norm_params* p, bool norm)
+{
+    if (!p) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no parameters");
+    if (p->batch < 0 || p->pixels < 0 || p->channels <= 0) return refuse(ADOP_ERR_INVALID_ARGUMENT, "batch, pixels or channels");
+    if (p->type != ADOP_TYPE_F32 && p->type != ADOP_TYPE_F16 && p->type != ADOP_TYPE_BF16)
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, "type is not ADOP_TYPE_*");
+    if (p->activation < ADOP_ACTIVATION_NONE || p->activation > ADOP_ACTIVATION_SILU)
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, "activation is not ADOP_ACTIVATION_*");
+    if (p->channels > ADOP_NORM_MAX_CHANNELS) return refuse(ADOP_ERR_SIZE_LIMIT, "more than ADOP_NORM_MAX_CHANNELS channels");
+    if (p->batch > 65535 || p->pixels > 0x7F000000)  // rows are counted with 32-bit ints
+        return refuse(ADOP_ERR_SIZE_LIMIT, "more than 65535 images, or 0x7F000000 pixels in one");
+    if (norm)
+    {
+        if (p->num_groups <= 0 || p->channels % p->num_groups != 0)
+            return refuse(ADOP_ERR_INVALID_ARGUMENT, "num_groups does not divide the channels");
+        if (p->param_type != ADOP_TYPE_F32 && p->param_type != p->type)
+            return refuse(ADOP_ERR_INVALID_ARGUMENT, "param_type is neither ADOP_TYPE_F32 nor the images' type");
+        if (!(p->eps >= 0.f) || p->eps > 3.0e38f) return refuse(ADOP_ERR_INVALID_ARGUMENT, "eps is negative or not finite");
+    }
+    return ADOP_OK;
+}
+
+constexpr int64_t kStrideLimit = (int64_t)1 << 40;  // keeps every offset below 2^63
+
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+adop_status check_image(const adop_norm_params* p, const adop_norm_image& im, bool output, const char* what)
+{
+    if (!im.data || !aligned(im.data, (size_t)element_size(p->type))) return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
+    if (im.image_stride < 0 || im.pixel_stride < 0 || im.image_stride > kStrideLimit || im.pixel_stride > kStrideLimit / (int64_t)65536)
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
+    if (output)
+    {
+        if (p->pixels > 1 && im.pixel_stride < p->channels) return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
+        if (p->batch > 1 && im.image_stride < (p->pixels - 1) * im.pixel_stride + p->channels) return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
+    }
+    return ADOP_OK;
+}
+
+// Vector and row of a call. The widest vector that every tensor's address and strides allow: 16 bytes, 8 bytes or one element.
+// A vector either lies within a pixel's channels, or all tensors are dense and a row of lcm(channels, vector) elements holds
+// whole pixels, an even number of times per image.
+struct Shape
+{
+    int vec, V, P, ppr;
+};
+Shape choose_shape(const adop_norm_params* p, const adop_norm_image* const* images, int n)
+{
+    const int es = element_size(p->type);
+    for (int vec = kVec16; vec <= kVec8; ++vec)
+    {
+        const int V = (vec == kVec16 ? 16 : 8) / es;
+        bool ok = true, dense = true;
+        for (int i = 0; i < n; ++i)
+        {
+            const adop_norm_image& im = *images[i];
+            ok = ok && aligned(im.data, (size_t)V * es) && (p->batch == 1 || im.image_stride % V == 0);
+            dense = dense && (p->pixels == 1 || im.pixel_stride == p->channels);
+        }
+        if (!ok) continue;
+        bool within = p->channels % V == 0;
+        for (int i = 0; i < n; ++i) within = within && (p->pixels == 1 || images[i]->pixel_stride % V == 0);
+        if (within) return {vec, V, p->channels / V, 1};
+        const int common = (int)gcd64(p->channels, V), ppr = V / common;
+        if (dense && p->pixels % ppr == 0 && (int64_t)p->channels * ppr <= ADOP_NORM_MAX_CHANNELS) return {vec, V, p->channels / common, ppr};
+    }
+    return {kVec1, 1, p->channels, 1};
+}
+
+// Blocks and threads of a launch over rows of P vectors: as many whole rows as `most` threads hold.
+void threads_of(int P, int most, int* R, int* threads)
+{
+    *R = P > most ? 1 : most / P;
+    *threads = P > most ? most : (*R * P + 31) / 32 * 32;
+}
+
+// Images whose inputs are read twice, by the sums and by what follows, are taken in groups that the L2 holds.
+constexpr int64_t kL2Group = 48ll << 20;
+constexpr int64_t kMinChunk = 16 << 10;  // bytes of one tensor that a block is worth
+
+// How the streaming kernels share out a batch: images of a launch and blocks of an image. By the sizes alone, so that the
+// workspace is known without the tensors.
+struct Share
+{
+    int images, chunks;
+};
+Share share_of(const adop_norm_params* p, bool gated, bool backward)
+{
+    const int64_t tensor = p->pixels * p->channels * element_size(p->type);
+    const int64_t read = tensor * (1 + (gated ? 1 : 0) + (backward ? 1 : 0));
+    int64_t images = kL2Group / (read > 0 ? read : 1);
+    if (images < 1) images = 1;
+    if (images > p->batch) images = p->batch;
+    const int64_t launches = (p->batch + images - 1) / images;
+    images = (p->batch + launches - 1) / launches;
+    const int64_t wave = (int64_t)sm_count() * (backward ? kNormGradBlocks : kNormBlocks);
+    int64_t chunks = wave / images, worth = (tensor + kMinChunk - 1) / kMinChunk;
+    if (chunks > worth) chunks = worth;
+    return {(int)images, (int)(chunks < 1 ? 1 : chunks)};
+}
+int cluster_of(int chunks) { return chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1; }
+
+constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
+size_t group_part_bytes(const adop_norm_params* p, int clusters) { return align16(sizeof(double2) * p->batch * (size_t)clusters * p->num_groups); }
+size_t channel_part_bytes(const adop_norm_params* p, int clusters) { return align16(sizeof(float2) * p->batch * (size_t)clusters * p->channels); }
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+struct Launch
+{
+    const char* name;
+    int which, threads, cluster;
+    dim3 grid;
+    size_t smem;
+    bool early;  // may start before the launch in front of it has ended (it waits by itself)
+};
+
+const void* kernel_of(int type, int which, int vec, bool gated, int act)
+{
+    if (type == ADOP_TYPE_F32) return norm_kernel_f32(which, vec, gated, act);
+    return type == ADOP_TYPE_F16 ? norm_kernel_f16(which, vec, gated, act) : norm_kernel_bf16(which, vec, gated, act);
+}
+
+adop_status launch(const Launch& l, const adop_norm_params* p, const Shape& sh, bool gated, NormArgs& a, cudaStream_t st)
+{
+    const void* f = kernel_of(p->type, l.which, sh.vec, gated, p->activation);
+    if (l.smem > 48 * 1024)
+    {
+        static OncePerDevice once[3][kNormKernels][kNormVectors][2][4];
+        int device = 0;
+        ADOP_CUDA_TRY(cudaGetDevice(&device));
+        ADOP_CUDA_TRY(once[p->type][l.which][sh.vec][gated][p->activation].run(
+            device, [&] { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }));
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = l.grid;
+    cfg.blockDim = dim3((unsigned)l.threads);
+    cfg.dynamicSmemBytes = l.smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)l.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = l.early ? 2 : 1;
+    void* args[] = {&a};
+    cudaError_t e = cudaSuccess;
+    ADOP_LAUNCH(l.name, st, (e = cudaLaunchKernelExC(&cfg, f, args)));
+    if (e != cudaSuccess) return record_cuda_error(e, l.name);
+    return ADOP_OK;
+}
+
+NormImage image_of(const adop_norm_image& im, const Shape& sh) { return {im.data, im.image_stride, im.pixel_stride * sh.ppr}; }
+
+NormArgs args_of(const adop_norm_params* p, const Shape& sh, bool norm)
+{
+    NormArgs a{};
+    a.C = p->channels;
+    a.G = norm ? p->num_groups : 1;
+    a.Cg = a.C / a.G;
+    a.slices = 1;
+    a.P = sh.P; a.ppr = sh.ppr;
+    a.rows = (int)(p->pixels / sh.ppr);
+    a.m = (int)gcd64(a.Cg, sh.V);
+    a.act = p->activation;
+    a.param_type = p->param_type;
+    a.eps = p->eps;
+    a.weight = p->weight; a.bias = p->bias;
+    return a;
+}
+int lanes_for(int items)
+{
+    int l = 1;
+    while (l < 32 && l < items) l *= 2;
+    return l;
+}
+// block_sums' scratch, as the kernel lays it out
+size_t sums_scratch(const Shape& sh, int m, int R, int threads)
+{
+    if (R == 1) return 0;
+    const int rows = 32 % sh.P == 0 ? threads / 32 : R;
+    return sizeof(float) * ((size_t)2 * (sh.V / m) * rows * sh.P + threads);
+}
+
+size_t apply_smem(int G, int threads) { return sizeof(double2) * (G + (G > threads ? G : threads)) + sizeof(float2) * G; }
+
+adop_status check_workspace(const adop_norm_params* p, const adop_norm_io* io, bool gated, bool backward)
+{
+    const size_t need = adop_group_norm_workspace_bytes(p, gated, backward);
+    if (need == 0) return ADOP_OK;
+    if (!io->workspace || io->workspace_bytes < need) return refuse(ADOP_ERR_WORKSPACE_TOO_SMALL, "workspace below adop_group_norm_workspace_bytes");
+    if (!aligned(io->workspace, 16)) return refuse(ADOP_ERR_INVALID_ARGUMENT, "the workspace is not 16-byte aligned");
+    return ADOP_OK;
+}
+
+#define ADOP_TRY(expr)                       \
+    do {                                     \
+        const adop_status _s = (expr);       \
+        if (_s != ADOP_OK) return _s;        \
+    } while (0)
+
+}  // namespace
+}  // namespace adop
+
+using namespace adop;
+
+extern "C" size_t adop_group_norm_workspace_bytes(const adop_norm_params* p, int32_t gated, int32_t backward)
+{
+    if (check_params(p, true) != ADOP_OK || p->batch == 0 || p->pixels == 0) return 0;
+    const Share s = share_of(p, gated != 0, backward != 0);
+    const int clusters = s.chunks < 8 ? 1 : s.chunks / 8;
+    return group_part_bytes(p, clusters) + (backward ? channel_part_bytes(p, clusters) : 0);
+}
+
+extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream)
+{
+    ADOP_TRY(check_params(p, true));
+    if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
+    if (!io->mean != !io->rstd) return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd are given together or not at all");
+    if (p->batch == 0 || p->pixels == 0) return ADOP_OK;
+    const bool gated = io->gate.data != nullptr;
+    ADOP_TRY(check_image(p, io->x, false, "x"));
+    if (gated) ADOP_TRY(check_image(p, io->gate, false, "gate"));
+    ADOP_TRY(check_image(p, io->y, true, "y"));
+    ADOP_TRY(check_workspace(p, io, gated, false));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const adop_norm_image* images[3] = {&io->x, &io->y, &io->gate};
+    const Shape sh = choose_shape(p, images, gated ? 3 : 2);
+    NormArgs a = args_of(p, sh, true);
+    a.x = image_of(io->x, sh);
+    a.gate = image_of(io->gate, sh);
+    a.y = image_of(io->y, sh);
+    a.mean = io->mean; a.rstd = io->rstd;
+    a.group_part = static_cast<double2*>(io->workspace);
+    int threads;
+    threads_of(a.P, kNormThreads, &a.R, &threads);
+    a.lanes = lanes_for(a.Cg / a.m * a.ppr);
+    const Share share = share_of(p, gated, false);
+    const int most = share.chunks < a.rows ? share.chunks : a.rows, k = cluster_of(most), chunks = most / k * k;
+    a.clusters = chunks / k;
+    const size_t slots = (size_t)a.P * (sh.V / a.m);
+    const size_t smem_stats = sizeof(double2) * a.G + sizeof(float) * 3 * slots + sums_scratch(sh, a.m, a.R, threads);
+    const size_t smem_apply = apply_smem(a.G, threads);
+    for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
+    {
+        const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
+        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, k, dim3((unsigned)chunks, n), smem_stats, a.image0 > 0}, p, sh, gated, a, st));
+        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, 1, dim3((unsigned)chunks, n), smem_apply, true}, p, sh, gated, a, st));
+    }
+    return ADOP_OK;
+}
+
+extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const adop_norm_io* io, void* stream)
+{
+    ADOP_TRY(check_params(p, true));
+    if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
+    if ((io->grad_weight && !aligned(io->grad_weight, 2)) || (io->grad_bias && !aligned(io->grad_bias, 2)))
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, "grad_weight or grad_bias");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->batch == 0 || p->pixels == 0)
+    {
+        const size_t bytes = (size_t)p->channels * element_size(p->param_type);
+        if (io->grad_weight) ADOP_CUDA_TRY(cudaMemsetAsync(io->grad_weight, 0, bytes, st));
+        if (io->grad_bias) ADOP_CUDA_TRY(cudaMemsetAsync(io->grad_bias, 0, bytes, st));
+        return ADOP_OK;
+    }
+    const bool gated = io->gate.data != nullptr;
+    if (!io->mean || !io->rstd) return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd of the forward call");
+    ADOP_TRY(check_image(p, io->x, false, "x"));
+    ADOP_TRY(check_image(p, io->grad_y, false, "grad_y"));
+    ADOP_TRY(check_image(p, io->grad_x, true, "grad_x"));
+    if (gated)
+    {
+        ADOP_TRY(check_image(p, io->gate, false, "gate"));
+        ADOP_TRY(check_image(p, io->grad_gate, true, "grad_gate"));
+    }
+    ADOP_TRY(check_workspace(p, io, gated, true));
+    const adop_norm_image* images[5] = {&io->x, &io->grad_y, &io->grad_x, &io->gate, &io->grad_gate};
+    const Shape sh = choose_shape(p, images, gated ? 5 : 3);
+    NormArgs a = args_of(p, sh, true);
+    a.x = image_of(io->x, sh);
+    a.gate = image_of(io->gate, sh);
+    a.dy = image_of(io->grad_y, sh);
+    a.dx = image_of(io->grad_x, sh);
+    a.dgate = image_of(io->grad_gate, sh);
+    a.mean = io->mean; a.rstd = io->rstd;
+    a.dweight = io->grad_weight; a.dbias = io->grad_bias;
+    int threads;
+    threads_of(a.P, kNormGradThreads, &a.R, &threads);
+    a.lanes = lanes_for(a.Cg);
+    const Share share = share_of(p, gated, true);
+    const int most = share.chunks < a.rows ? share.chunks : a.rows, k = cluster_of(most), chunks = most / k * k;
+    a.clusters = chunks / k;
+    const bool params = io->grad_weight || io->grad_bias;
+    a.group_part = static_cast<double2*>(io->workspace);
+    a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.clusters)) : nullptr;
+    a.param_parts = p->batch * a.clusters;
+    const size_t smem_sums = sizeof(double2) * a.G + sizeof(float) * (2 * (size_t)a.C + 2 * (size_t)a.P * sh.V) + sums_scratch(sh, 1, a.R, threads);
+    size_t smem_apply = apply_smem(a.G, threads);
+    if (params && smem_apply < sizeof(double) * 2 * threads) smem_apply = sizeof(double) * 2 * threads;
+    for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
+    {
+        const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
+        // the parameters' gradients need the sums of all images: blocks of the last launch add them up
+        a.param_blocks = params && a.image0 + share.images >= p->batch ? (a.C + 31) / 32 : 0;
+        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, k, dim3((unsigned)chunks, n), smem_sums, a.image0 > 0}, p, sh, gated, a, st));
+        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, 1, dim3((unsigned)(chunks + a.param_blocks), n), smem_apply, true}, p, sh, gated, a, st));
+    }
+    return ADOP_OK;
+}
+
+namespace {
+adop_status gate_launch(const adop_norm_params* p, const Shape& sh, NormArgs& a, bool backward, cudaStream_t st)
+{
+    const int most = backward ? kNormGradThreads : kNormThreads;
+    int threads;
+    threads_of(a.P, most, &a.R, &threads);
+    const int64_t worth = (p->pixels * p->channels * element_size(p->type) + kMinChunk - 1) / kMinChunk;
+    int64_t chunks = ((int64_t)sm_count() * (backward ? kNormGradBlocks : kNormBlocks) + p->batch - 1) / p->batch;
+    if (chunks > worth) chunks = worth;
+    if (chunks > a.rows) chunks = a.rows;
+    return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, 1, dim3((unsigned)chunks, (unsigned)p->batch), 0, false}, p, sh,
+                  true, a, st);
+}
+}  // namespace
+
+extern "C" adop_status adop_gated_activation_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream)
+{
+    ADOP_TRY(check_params(p, false));
+    if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
+    if (p->batch == 0 || p->pixels == 0) return ADOP_OK;
+    ADOP_TRY(check_image(p, io->x, false, "x"));
+    ADOP_TRY(check_image(p, io->gate, false, "gate"));
+    ADOP_TRY(check_image(p, io->y, true, "y"));
+    const adop_norm_image* images[3] = {&io->x, &io->gate, &io->y};
+    const Shape sh = choose_shape(p, images, 3);
+    NormArgs a = args_of(p, sh, false);
+    a.x = image_of(io->x, sh);
+    a.gate = image_of(io->gate, sh);
+    a.y = image_of(io->y, sh);
+    return gate_launch(p, sh, a, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" adop_status adop_gated_activation_backward(const adop_norm_params* p, const adop_norm_io* io, void* stream)
+{
+    ADOP_TRY(check_params(p, false));
+    if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
+    if (p->batch == 0 || p->pixels == 0) return ADOP_OK;
+    ADOP_TRY(check_image(p, io->x, false, "x"));
+    ADOP_TRY(check_image(p, io->gate, false, "gate"));
+    ADOP_TRY(check_image(p, io->grad_y, false, "grad_y"));
+    ADOP_TRY(check_image(p, io->grad_x, true, "grad_x"));
+    ADOP_TRY(check_image(p, io->grad_gate, true, "grad_gate"));
+    const adop_norm_image* images[5] = {&io->x, &io->gate, &io->grad_y, &io->grad_x, &io->grad_gate};
+    const Shape sh = choose_shape(p, images, 5);
+    NormArgs a = args_of(p, sh, false);
+    a.x = image_of(io->x, sh);
+    a.gate = image_of(io->gate, sh);
+    a.dy = image_of(io->grad_y, sh);
+    a.dx = image_of(io->grad_x, sh);
+    a.dgate = image_of(io->grad_gate, sh);
+    return gate_launch(p, sh, a, true, static_cast<cudaStream_t>(stream));
+}

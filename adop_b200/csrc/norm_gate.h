@@ -1,0 +1,66 @@
+// Group normalisation with an activation and the gate of a gated convolution on channels-last images: what the host side
+// (norm_gate.cu) and the kernels (norm_gate.cuh, compiled once per image type) share.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace adop {
+
+enum NormKernel
+{
+    kNormStats,         // sums of u and u^2 per group
+    kNormApply,         // y = act((u - mean) rstd w + b)
+    kNormGradSums,      // per channel: sums of dz and dz uhat
+    kNormGradApply,     // dx, and the parameters' gradients from the sums
+    kNormResident,      // forward pass of images that fit a cluster's shared memory
+    kNormGradResident,  // backward pass of such images
+    kNormGradParams,    // the parameters' gradients behind kNormGradResident
+    kGate,              // y = act(f) sigmoid(g)
+    kGateGrad,          // df, dg
+    kNormKernels
+};
+enum NormVector { kVec16, kVec8, kVec1, kNormVectors };  // bytes of a thread's vector; kVec1 = one element
+constexpr int kNormActs = 5;                             // 0..3 = ADOP_ACTIVATION_*, 4 = chosen at run time
+
+// One channels-last tensor: element (b, pixel, c) at p + b * image + pixel * (row / pixels per row) + c; strides in elements.
+struct NormImage
+{
+    const void* p;
+    int64_t image, row;
+};
+
+// An image is walked in rows of P vectors: P vectors of VEC elements are the smallest run that starts and ends with a pixel,
+// so a thread that moves on by whole rows keeps its channels, and with them its coefficients and its sums, in registers.
+struct NormArgs
+{
+    int C, G, Cg;     // channels and groups of a slice; channels of a group
+    int slices;       // independent channel ranges of an image (1 but in the resident kernels)
+    int P, ppr;       // vectors and pixels of a row
+    int R;            // rows that a block takes at once (1 when a row has more vectors than the block threads)
+    int m;            // channels of a thread's vector that share a group: gcd(Cg, VEC)
+    int lanes;        // threads that add up one group's slots (a power of two up to 32)
+    int rows;         // rows of an image
+    int image0;       // first image of the launch
+    int clusters;     // partial sums of an image
+    int param_blocks; // blocks of kNormGradApply that add up the parameters' gradients
+    int param_parts;  // partial sums of a channel, over all images
+    int act, param_type;
+    float eps;
+    NormImage x, gate, y, dy, dx, dgate;
+    const void *weight, *bias;
+    void *dweight, *dbias;
+    float *mean, *rstd;   // [B, slices * G]
+    double2* group_part;  // [B, clusters, G]
+    float2* channel_part; // [B, clusters, C] (resident: [B, 1, slices * C])
+};
+
+// threads of a block and resident blocks of an SM that the kernels are compiled for
+constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
+constexpr int kNormGradThreads = 256, kNormGradBlocks = 2;  // backward
+constexpr int kNormMaxThreads = 512;
+
+const void* norm_kernel_f32(int which, int vec, bool gated, int act);
+const void* norm_kernel_f16(int which, int vec, bool gated, int act);
+const void* norm_kernel_bf16(int which, int vec, bool gated, int act);
+
+}  // namespace adop

@@ -6,6 +6,8 @@
 //   BlendPointCloud              (PointRenderer.h:52, RenderInfo.cpp:19-31)                        -> adop::blend_point_cloud
 //   ApplyTangentToPose           (PointRenderer.h:63)                                              -> adop::apply_tangent_to_pose
 //   NeuralCameraImpl::forward    (src/lib/models/NeuralCamera.h:128-129)                          -> adop::tonemap (adop::Tonemap)
+// and what stands between the convolutions of the gated blocks that the reference's U-Net is built of (src/lib/models/Pipeline.h:134-135):
+//   adop::group_norm, adop::gated_activation, adop::gated_group_norm (adop::GroupNorm, adop::GatedActivation)
 // Same differentiable inputs in the same order (texture [C,N], background [C], points [N,4], pose tangents [I,6] f64,
 // intrinsics [K,cols]), same outputs (L colour tensors, then L masks when requested), gradients in the same order.
 // The reference's NeuralRenderInfo points at a NeuralScene (which needs the whole saiga library); RenderInfo carries the
@@ -16,6 +18,8 @@
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+
+#include <limits>
 
 #include "adop/adop_raster.h"
 
@@ -480,6 +484,221 @@ static Tensor tonemap(Tensor x, c10::optional<Tensor> frame_index, c10::optional
                           image_w, image_h, leak);
 }
 
+// ---- operators of the rendering network: channels-last images [B,C,H,W] in float32, float16 or bfloat16 ---------------------
+// adop::group_norm        y = act(group_norm(x) weight + bias)
+// adop::gated_activation  y = act(f) sigmoid(g), x [B,2C,H,W] = features f, then gates g: what the two convolutions of a gated block
+//                         put out, as one convolution with twice the channels does
+// adop::gated_group_norm  y = group_norm(act(f) sigmoid(g)) weight + bias
+// A channel range of a wider channels-last image is taken as it is; any other order is copied to channels-last first. Outputs and
+// gradients of images are dense channels-last.
+static int32_t type_of(const Tensor& t, const char* what)
+{
+    switch (t.scalar_type())
+    {
+        case torch::kFloat32: return ADOP_TYPE_F32;
+        case torch::kFloat16: return ADOP_TYPE_F16;
+        case torch::kBFloat16: return ADOP_TYPE_BF16;
+        default: TORCH_CHECK(false, what, ": float32, float16 or bfloat16, not ", t.scalar_type());
+    }
+}
+static int64_t activation_of(const std::string& name)
+{
+    if (name == "none") return ADOP_ACTIVATION_NONE;
+    if (name == "relu") return ADOP_ACTIVATION_RELU;
+    if (name == "elu") return ADOP_ACTIVATION_ELU;
+    if (name == "silu") return ADOP_ACTIVATION_SILU;
+    TORCH_CHECK(false, "activation is none, relu, elu or silu, not ", name);
+}
+// whether the pixels of t [B,C,H,W] lie at one stride with their channels side by side, and that stride
+static bool pixel_stride(const Tensor& t, int64_t* stride)
+{
+    const int64_t C = t.size(1), H = t.size(2), W = t.size(3);
+    *stride = W > 1 ? t.stride(3) : (H > 1 ? t.stride(2) : C);
+    return (C == 1 || t.stride(1) == 1) && (H <= 1 || W <= 1 || t.stride(2) == W * t.stride(3));
+}
+static Tensor channels_last(const Tensor& t)
+{
+    int64_t stride;
+    return t.numel() == 0 || pixel_stride(t, &stride) ? t : t.contiguous(torch::MemoryFormat::ChannelsLast);
+}
+// channels [c0, ...) of t
+static adop_norm_image norm_image(const Tensor& t, int64_t c0 = 0)
+{
+    adop_norm_image im{};
+    if (t.numel() == 0) return im;
+    TORCH_CHECK(pixel_stride(t, &im.pixel_stride), "the image is not in channels-last order");
+    im.image_stride = t.size(0) > 1 ? t.stride(0) : 0;
+    im.data = static_cast<char*>(t.data_ptr()) + c0 * t.element_size();
+    return im;
+}
+static Tensor new_image(const Tensor& like, int64_t channels)
+{
+    return torch::empty({like.size(0), channels, like.size(2), like.size(3)}, like.options().memory_format(torch::MemoryFormat::ChannelsLast));
+}
+static adop_norm_params norm_params(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps, int64_t activation, bool gated)
+{
+    TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
+    adop_norm_params p{};
+    p.type = type_of(x, "x");
+    TORCH_CHECK(!gated || x.size(1) % 2 == 0, "x of a gated operator has features and as many gates");
+    const int64_t C = gated ? x.size(1) / 2 : x.size(1);
+    const int64_t limit = std::numeric_limits<int32_t>::max();
+    TORCH_CHECK(x.size(0) <= limit && C <= limit && groups <= limit && groups >= 0, "sizes beyond 32 bits");
+    p.batch = (int32_t)x.size(0); p.channels = (int32_t)C; p.pixels = x.size(2) * x.size(3);
+    p.num_groups = (int32_t)groups; p.activation = (int32_t)activation; p.eps = (float)eps;
+    p.param_type = ADOP_TYPE_F32;
+    const Tensor& one = weight.defined() ? weight : bias;
+    if (one.defined()) p.param_type = type_of(one, "weight and bias");
+    for (const Tensor* t : {&weight, &bias})
+        if (t->defined())
+            TORCH_CHECK(t->device() == x.device() && t->dim() == 1 && t->size(0) == C && t->is_contiguous() && type_of(*t, "weight and bias") == p.param_type,
+                        "weight and bias: contiguous [C] of one type on x's device");
+    if (weight.defined()) p.weight = weight.data_ptr();
+    if (bias.defined()) p.bias = bias.data_ptr();
+    return p;
+}
+static Tensor norm_workspace(const adop_norm_params& p, bool gated, bool backward, const Tensor& x, adop_norm_io* io)
+{
+    const size_t bytes = adop_group_norm_workspace_bytes(&p, gated, backward);
+    if (bytes == 0) return Tensor();
+    Tensor ws = torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8).memory_format(torch::MemoryFormat::Contiguous));
+    io->workspace = ws.data_ptr();
+    io->workspace_bytes = bytes;
+    return ws;
+}
+// x in channels-last order; stats: [2,B,G] float32 for mean and rstd, or undefined
+static Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps, int64_t activation, bool gated,
+                                 const Tensor& stats)
+{
+    const adop_norm_params p = norm_params(x, weight, bias, groups, eps, activation, gated);
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = new_image(x, p.channels);
+    adop_norm_io io{};
+    io.x = norm_image(x);
+    if (gated) io.gate = norm_image(x, p.channels);
+    io.y = norm_image(y);
+    if (stats.defined() && stats.numel() > 0)
+    {
+        io.mean = stats.data_ptr<float>();
+        io.rstd = io.mean + stats.numel() / 2;
+    }
+    Tensor ws = norm_workspace(p, gated, false, x, &io);
+    check_status(adop_group_norm_forward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_group_norm_forward");
+    return y;
+}
+static bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
+static void once_differentiable(const char* what)
+{
+    TORCH_CHECK(!torch::GradMode::is_enabled(), what, " has no second derivative: its gradients cannot be recorded (create_graph)");
+}
+
+struct GroupNorm : public torch::autograd::Function<GroupNorm>
+{
+    static Variable forward(AutogradContext* ctx, Variable x, c10::optional<Tensor> weight_, c10::optional<Tensor> bias_, int64_t groups, double eps,
+                            int64_t activation, bool gated)
+    {
+        const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
+        Tensor stats = torch::empty({2, x.size(0), groups}, x.options().dtype(torch::kFloat32).memory_format(torch::MemoryFormat::Contiguous));
+        Tensor y = group_norm_forward(x, weight, bias, groups, eps, activation, gated, stats);
+        ctx->save_for_backward({x, weight, bias, stats});
+        ctx->saved_data["groups"] = groups; ctx->saved_data["eps"] = eps; ctx->saved_data["activation"] = activation;
+        ctx->saved_data["gated"] = gated;
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grad_output)
+    {
+        once_differentiable("group_norm");
+        auto saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+        const bool gated = ctx->saved_data["gated"].toBool();
+        const adop_norm_params p = norm_params(x, weight, bias, ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
+                                               ctx->saved_data["activation"].toInt(), gated);
+        c10::cuda::CUDAGuard guard(x.device());
+        Tensor dy = channels_last(grad_output[0]), dx = new_image(x, x.size(1)), dw, db;
+        adop_norm_io io{};
+        io.x = norm_image(x);
+        io.grad_y = norm_image(dy);
+        io.grad_x = norm_image(dx);
+        if (gated) { io.gate = norm_image(x, p.channels); io.grad_gate = norm_image(dx, p.channels); }
+        if (stats.numel() > 0)
+        {
+            io.mean = stats.data_ptr<float>();
+            io.rstd = io.mean + stats.numel() / 2;
+        }
+        if (wants_gradient(weight)) { dw = torch::empty_like(weight); io.grad_weight = dw.data_ptr(); }
+        if (wants_gradient(bias)) { db = torch::empty_like(bias); io.grad_bias = db.data_ptr(); }
+        Tensor ws = norm_workspace(p, gated, true, x, &io);
+        check_status(adop_group_norm_backward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_group_norm_backward");
+        return {dx, dw, db, Variable(), Variable(), Variable(), Variable()};
+    }
+};
+
+static Tensor group_norm_call(const Tensor& x, int64_t groups, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps,
+                              const std::string& activation, bool gated)
+{
+    TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
+    TORCH_CHECK(groups > 0, "num_groups is positive");
+    const int64_t act = activation_of(activation);
+    const Tensor xc = channels_last(x), w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
+    if (torch::GradMode::is_enabled() && (wants_gradient(x) || wants_gradient(w) || wants_gradient(b)))
+        return GroupNorm::apply(xc, weight, bias, groups, eps, act, gated);
+    return group_norm_forward(xc, w, b, groups, eps, act, gated, Tensor());
+}
+static Tensor group_norm(const Tensor& x, int64_t num_groups, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps,
+                         std::string activation)
+{
+    return group_norm_call(x, num_groups, weight, bias, eps, activation, false);
+}
+static Tensor gated_group_norm(const Tensor& x, int64_t num_groups, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps,
+                               std::string activation)
+{
+    return group_norm_call(x, num_groups, weight, bias, eps, activation, true);
+}
+
+static Tensor gated_forward(const Tensor& x, int64_t activation)
+{
+    const adop_norm_params p = norm_params(x, Tensor(), Tensor(), 0, 0.0, activation, true);
+    c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = new_image(x, p.channels);
+    adop_norm_io io{};
+    io.x = norm_image(x);
+    io.gate = norm_image(x, p.channels);
+    io.y = norm_image(y);
+    check_status(adop_gated_activation_forward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_gated_activation_forward");
+    return y;
+}
+struct GatedActivation : public torch::autograd::Function<GatedActivation>
+{
+    static Variable forward(AutogradContext* ctx, Variable x, int64_t activation)
+    {
+        ctx->save_for_backward({x});
+        ctx->saved_data["activation"] = activation;
+        return gated_forward(x, activation);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grad_output)
+    {
+        once_differentiable("gated_activation");
+        const Tensor x = ctx->get_saved_variables()[0];
+        const adop_norm_params p = norm_params(x, Tensor(), Tensor(), 0, 0.0, ctx->saved_data["activation"].toInt(), true);
+        c10::cuda::CUDAGuard guard(x.device());
+        Tensor dy = channels_last(grad_output[0]), dx = new_image(x, x.size(1));
+        adop_norm_io io{};
+        io.x = norm_image(x); io.gate = norm_image(x, p.channels);
+        io.grad_y = norm_image(dy);
+        io.grad_x = norm_image(dx); io.grad_gate = norm_image(dx, p.channels);
+        check_status(adop_gated_activation_backward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_gated_activation_backward");
+        return {dx, Variable()};
+    }
+};
+static Tensor gated_activation(const Tensor& x, std::string activation)
+{
+    TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,2C,H,W]");
+    const int64_t act = activation_of(activation);
+    const Tensor xc = channels_last(x);
+    if (torch::GradMode::is_enabled() && wants_gradient(x)) return GatedActivation::apply(xc, act);
+    return gated_forward(xc, act);
+}
+
 }  // namespace adop
 
 TORCH_LIBRARY(adop, m)
@@ -495,4 +714,7 @@ TORCH_LIBRARY(adop, m)
     m.def("blend_point_cloud_environment", &adop::blend_point_cloud_environment);
     m.def("apply_tangent_to_pose", &adop::apply_tangent_to_pose);
     m.def("tonemap", &adop::tonemap);
+    m.def("group_norm(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str activation=\"none\") -> Tensor", &adop::group_norm);
+    m.def("gated_activation(Tensor x, str activation=\"elu\") -> Tensor", &adop::gated_activation);
+    m.def("gated_group_norm(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-05, str activation=\"elu\") -> Tensor", &adop::gated_group_norm);
 }

@@ -472,6 +472,69 @@ adop_status adop_tonemap_forward(const adop_tonemap_params* p, const float* x, f
 adop_status adop_tonemap_backward(const adop_tonemap_params* p, const float* x, const float* grad_out,
                                   adop_tonemap_grads* g, void* stream);
 
+/* ---- operators of the rendering network between the rasterizer and the tonemapper --------------------------------------
+ * The reference feeds the pyramid to a U-Net of gated convolution blocks (src/lib/models/Pipeline.h:134-135;
+ * configs/train_boat.ini:132-148), in channels-last order and half precision where asked for (Pipeline.cpp:200-224). The
+ * convolutions stay with the library that the host program uses; what stands between them is here, each as one pass over
+ * the image where it fits on the chip:
+ *   adop_group_norm        y = act((x - mean) rstd w + b), or with a gate image, y = (u - mean) rstd w + b for the output
+ *                          u = act(x) sigmoid(gate) of a gated convolution; mean and rstd over the pixels and channels of a
+ *                          group, rstd = 1 / sqrt(var + eps), var without Bessel's correction
+ *   adop_gated_activation  y = act(x) sigmoid(gate)
+ * Images are channels-last with any pixel and image stride (a channel range of a wider image is one). Statistics and sums are
+ * kept in 32 bits or more and every output is rounded once. Same inputs, same bits. */
+#define ADOP_TYPE_F32 0
+#define ADOP_TYPE_F16 1
+#define ADOP_TYPE_BF16 2
+
+#define ADOP_ACTIVATION_NONE 0
+#define ADOP_ACTIVATION_RELU 1
+#define ADOP_ACTIVATION_ELU 2 /* alpha = 1 */
+#define ADOP_ACTIVATION_SILU 3
+
+#define ADOP_NORM_MAX_CHANNELS 4096
+
+/* Element (b, pixel, c) at data[b * image_stride + pixel * pixel_stride + c]; strides in elements. Inputs may repeat images
+ * or pixels (stride 0); the pixels of an output must not overlap, and outputs share no memory with inputs or one another. */
+typedef struct adop_norm_image
+{
+    void* data;
+    int64_t image_stride, pixel_stride;
+} adop_norm_image;
+
+typedef struct adop_norm_params
+{
+    int32_t batch, channels;
+    int64_t pixels;     /* of an image: height * width, up to 0x7F000000 */
+    int32_t num_groups; /* divides channels; not read by adop_gated_activation_* */
+    int32_t type;       /* of all images, ADOP_TYPE_* */
+    int32_t param_type; /* of weight, bias and their gradients: ADOP_TYPE_F32 or `type` */
+    int32_t activation; /* ADOP_ACTIVATION_* */
+    float eps;          /* >= 0 */
+    const void* weight; /* [channels] or NULL = 1 */
+    const void* bias;   /* [channels] or NULL = 0 */
+} adop_norm_params;
+
+typedef struct adop_norm_io
+{
+    adop_norm_image x, gate;  /* [batch, pixels, channels]; group norm: gate.data = NULL without a gate */
+    adop_norm_image y;        /* forward: the result */
+    float *mean, *rstd;       /* group norm [batch, num_groups]: forward writes them (both, or NULL), backward reads them */
+    adop_norm_image grad_y;   /* backward */
+    adop_norm_image grad_x, grad_gate; /* backward; grad_gate.data = NULL without a gate */
+    void *grad_weight, *grad_bias;     /* backward, [channels] or NULL; overwritten */
+    void* workspace;          /* group norm: adop_group_norm_workspace_bytes, 16-byte aligned; contents need not survive */
+    size_t workspace_bytes;
+} adop_norm_io;
+
+/* Bytes of workspace that a group norm call makes use of on the current device, with or without a gate image; 0 for
+ * arguments that the call refuses, and where it needs none. */
+size_t adop_group_norm_workspace_bytes(const adop_norm_params* p, int32_t gated, int32_t backward);
+adop_status adop_group_norm_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream);
+adop_status adop_group_norm_backward(const adop_norm_params* p, const adop_norm_io* io, void* stream);
+adop_status adop_gated_activation_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream);
+adop_status adop_gated_activation_backward(const adop_norm_params* p, const adop_norm_io* io, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

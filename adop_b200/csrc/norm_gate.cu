@@ -68,10 +68,10 @@ struct Shape
 {
     int vec, V, P, ppr;
 };
-Shape choose_shape(const adop_norm_params* p, const adop_norm_image* const* images, int n)
+Shape choose_shape(const adop_norm_params* p, const adop_norm_image* const* images, int n, int from = kVec16)
 {
     const int es = element_size(p->type);
-    for (int vec = kVec16; vec <= kVec8; ++vec)
+    for (int vec = from; vec <= kVec8; ++vec)
     {
         const int V = (vec == kVec16 ? 16 : 8) / es;
         bool ok = true, dense = true;
@@ -99,7 +99,7 @@ void threads_of(int P, int most, int* R, int* threads)
 }
 
 // Images whose inputs are read twice, by the sums and by what follows, are taken in groups that the L2 holds.
-constexpr int64_t kL2Group = 48ll << 20;
+constexpr int64_t kL2Group = 64ll << 20;
 constexpr int64_t kMinChunk = 16 << 10;  // bytes of one tensor that a block is worth
 
 // How the streaming kernels share out a batch: images of a launch and blocks of an image. By the sizes alone, so that the
@@ -117,16 +117,68 @@ Share share_of(const adop_norm_params* p, bool gated, bool backward)
     if (images > p->batch) images = p->batch;
     const int64_t launches = (p->batch + images - 1) / images;
     images = (p->batch + launches - 1) / launches;
-    const int64_t wave = (int64_t)sm_count() * (backward ? kNormGradBlocks : kNormBlocks);
+    const int64_t wave = (int64_t)sm_count();
     int64_t chunks = wave / images, worth = (tensor + kMinChunk - 1) / kMinChunk;
     if (chunks > worth) chunks = worth;
     return {(int)images, (int)(chunks < 1 ? 1 : chunks)};
 }
-int cluster_of(int chunks) { return chunks >= 8 ? 8 : chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1; }
 
 constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
-size_t group_part_bytes(const adop_norm_params* p, int clusters) { return align16(sizeof(double2) * p->batch * (size_t)clusters * p->num_groups); }
-size_t channel_part_bytes(const adop_norm_params* p, int clusters) { return align16(sizeof(float2) * p->batch * (size_t)clusters * p->channels); }
+size_t group_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->num_groups); }
+size_t channel_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->channels); }
+
+// ---- images that stay in shared memory --------------------------------------------------------------------------------------
+// A cluster of `k` blocks takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side.
+constexpr int64_t kSliceBytes = 64;
+struct Resident
+{
+    int slices, k, threads, R;  // slices: log2
+    size_t fixed, smem;  // bytes in front of the vectors, and in all
+};
+// block_sums' scratch, as the kernel lays it out
+size_t sums_scratch(const Shape& sh, int m, int R, int threads)
+{
+    return sizeof(float) * 2 * (size_t)(sh.V / m) * (32 % sh.P == 0 ? threads / 32 : R) * sh.P;
+}
+bool resident_of(const adop_norm_params* p, const Shape& sh, bool gated, bool backward, Resident* r)
+{
+    if (sh.vec == kVec1) return false;
+    const int es = element_size(p->type), tensors = 1 + (gated ? 1 : 0) + (backward ? 1 : 0), most = backward ? kNormGradThreads : kNormThreads;
+    const int64_t image = p->pixels * p->channels * es * tensors, cap = 96 << 10, least = 16 << 10;
+    const int64_t want = sm_count();
+    if (image > cap * 8 * p->num_groups) return false;
+    // the fewest blocks that hold the image; then more while there are fewer blocks than SMs and each has something to do
+    bool found = false;
+    for (int log2 = 0; log2 <= 6 && 1 << log2 <= p->num_groups; ++log2)
+    {
+        const int slices = 1 << log2;
+        if (p->num_groups % slices != 0) break;
+        const int C = p->channels / slices;
+        if (slices > 1 && (sh.ppr != 1 || C % sh.V != 0 || (int64_t)C * es < kSliceBytes || (int64_t)p->batch * slices > 65535)) break;
+        const int64_t part = image / slices, rows = p->pixels / sh.ppr;
+        for (int k = 1; k <= 8 && k <= rows; k *= 2)
+        {
+            Shape s = sh;
+            s.P = sh.P / slices;
+            if (s.P > most) continue;
+            Resident c{log2, k};
+            threads_of(s.P, most, &c.R, &c.threads);
+            const int G = p->num_groups / slices, m = (int)gcd64(p->channels / p->num_groups, sh.V);
+            const int64_t here = (rows + k - 1) / k, vectors = (here + c.R - 1) / c.R * c.threads * sh.V * es * tensors;
+            if (vectors > cap) continue;
+            if (found && ((int64_t)p->batch << r->slices) * r->k >= want) return true;
+            if (found && part / k < least) return true;
+            c.fixed = sizeof(double2) * G + sizeof(float2) * 2 * G + sums_scratch(s, backward ? 1 : m, c.R, c.threads) +
+                      sizeof(float) * (2 * (size_t)C + (backward ? 2 * (size_t)C : (size_t)s.P * (sh.V / m)));
+            c.fixed = align16(c.fixed);
+            c.smem = c.fixed + (size_t)vectors;
+            if (c.smem > 200 * 1024) continue;
+            *r = c;
+            found = true;
+        }
+    }
+    return found;
+}
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 struct Launch
@@ -183,7 +235,6 @@ NormArgs args_of(const adop_norm_params* p, const Shape& sh, bool norm)
     a.C = p->channels;
     a.G = norm ? p->num_groups : 1;
     a.Cg = a.C / a.G;
-    a.slices = 1;
     a.P = sh.P; a.ppr = sh.ppr;
     a.rows = (int)(p->pixels / sh.ppr);
     a.m = (int)gcd64(a.Cg, sh.V);
@@ -193,21 +244,36 @@ NormArgs args_of(const adop_norm_params* p, const Shape& sh, bool norm)
     a.weight = p->weight; a.bias = p->bias;
     return a;
 }
-int lanes_for(int items)
+// what follows from the sizes of a slice, the threads and the number of parts of an image
+void finish(NormArgs* a, int threads, int chunks)
 {
-    int l = 1;
-    while (l < 32 && l < items) l *= 2;
-    return l;
+    auto log2_of = [](int64_t items) {
+        int l = 0;
+        while (l < 5 && (1 << l) < items) ++l;
+        return l;
+    };
+    const int rows = 32 % a->P == 0 ? threads / 32 : a->R;
+    a->row_lanes = log2_of(rows);
+    a->lanes = log2_of((int64_t)(1 << a->row_lanes) * (a->Cg / a->m * a->ppr));
+    a->chunks = chunks;
+    a->chunk_rows = a->rows / chunks;
+    a->chunk_more = a->rows % chunks;
+    const double per_row = (double)a->ppr * a->Cg;
+    a->inv_n = 1.0 / (a->rows * per_row);
+    a->inv_short = 1.0 / (a->chunk_rows * per_row);
+    a->inv_long = 1.0 / ((a->chunk_rows + 1) * per_row);
+    a->inv_P = 1.f / a->P; a->inv_Cg = 1.f / a->Cg;
+    a->gather = log2_of(chunks);
+    while (a->gather > 0 && a->G << a->gather > threads) --a->gather;
 }
-// block_sums' scratch, as the kernel lays it out
-size_t sums_scratch(const Shape& sh, int m, int R, int threads)
-{
-    if (R == 1) return 0;
-    const int rows = 32 % sh.P == 0 ? threads / 32 : R;
-    return sizeof(float) * ((size_t)2 * (sh.V / m) * rows * sh.P + threads);
-}
+size_t apply_smem(const NormArgs& a) { return sizeof(float2) * 2 * a.G + sizeof(float) * 2 * a.C; }
 
-size_t apply_smem(int G, int threads) { return sizeof(double2) * (G + (G > threads ? G : threads)) + sizeof(float2) * G; }
+// the streaming kernels' vectors behind `fixed` bytes of shared memory; all in all
+size_t stream_smem(size_t fixed, const Shape& sh, int es, int threads, bool gated, bool grad)
+{
+    const int tensors = 1 + (gated ? 1 : 0) + (grad ? 1 : 0);
+    return align16(fixed) + (sh.vec == kVec1 ? 0 : (size_t)stream_depth(gated, grad) * tensors * threads * sh.V * es);
+}
 
 adop_status check_workspace(const adop_norm_params* p, const adop_norm_io* io, bool gated, bool backward)
 {
@@ -229,12 +295,25 @@ adop_status check_workspace(const adop_norm_params* p, const adop_norm_io* io, b
 
 using namespace adop;
 
+namespace {
+// the launch of a resident kernel: what a slice is to it
+NormArgs slice_args(const NormArgs& whole, const Resident& r)
+{
+    NormArgs a = whole;
+    a.slices = r.slices;
+    a.C >>= r.slices; a.G >>= r.slices; a.P >>= r.slices;
+    a.R = r.R;
+    finish(&a, r.threads, r.k);
+    a.vectors = (int)r.fixed;
+    return a;
+}
+}  // namespace
+
 extern "C" size_t adop_group_norm_workspace_bytes(const adop_norm_params* p, int32_t gated, int32_t backward)
 {
     if (check_params(p, true) != ADOP_OK || p->batch == 0 || p->pixels == 0) return 0;
     const Share s = share_of(p, gated != 0, backward != 0);
-    const int clusters = s.chunks < 8 ? 1 : s.chunks / 8;
-    return group_part_bytes(p, clusters) + (backward ? channel_part_bytes(p, clusters) : 0);
+    return group_part_bytes(p, s.chunks) + (backward ? channel_part_bytes(p, s.chunks) : 0);
 }
 
 extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream)
@@ -256,21 +335,29 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     a.gate = image_of(io->gate, sh);
     a.y = image_of(io->y, sh);
     a.mean = io->mean; a.rstd = io->rstd;
-    a.group_part = static_cast<double2*>(io->workspace);
+    a.group_part = static_cast<float2*>(io->workspace);
+    Resident r;
+    if (resident_of(p, sh, gated, false, &r))
+    {
+        NormArgs s = slice_args(a, r);
+        return launch({"k_norm_resident", kNormResident, r.threads, r.k, dim3((unsigned)r.k, (unsigned)p->batch << r.slices), r.smem, false}, p, sh, gated, s, st);
+    }
     int threads;
     threads_of(a.P, kNormThreads, &a.R, &threads);
-    a.lanes = lanes_for(a.Cg / a.m * a.ppr);
     const Share share = share_of(p, gated, false);
-    const int most = share.chunks < a.rows ? share.chunks : a.rows, k = cluster_of(most), chunks = most / k * k;
-    a.clusters = chunks / k;
-    const size_t slots = (size_t)a.P * (sh.V / a.m);
-    const size_t smem_stats = sizeof(double2) * a.G + sizeof(float) * 3 * slots + sums_scratch(sh, a.m, a.R, threads);
-    const size_t smem_apply = apply_smem(a.G, threads);
+    finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
+    const size_t smem_stats = sizeof(float) * a.P * (sh.V / a.m) + sums_scratch(sh, a.m, a.R, threads);
+    const size_t smem_apply = apply_smem(a);
+    const int es = element_size(p->type);
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
     {
         const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
-        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, k, dim3((unsigned)chunks, n), smem_stats, a.image0 > 0}, p, sh, gated, a, st));
-        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, 1, dim3((unsigned)chunks, n), smem_apply, true}, p, sh, gated, a, st));
+        a.vectors = (int)align16(smem_stats);
+        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_stats, sh, es, threads, gated, false), a.image0 > 0}, p,
+                        sh, gated, a, st));
+        a.vectors = (int)align16(smem_apply);
+        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_apply, sh, es, threads, gated, false), true}, p, sh,
+                        gated, a, st));
     }
     return ADOP_OK;
 }
@@ -310,26 +397,41 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
     a.dgate = image_of(io->grad_gate, sh);
     a.mean = io->mean; a.rstd = io->rstd;
     a.dweight = io->grad_weight; a.dbias = io->grad_bias;
+    const bool params = io->grad_weight || io->grad_bias;
+    Resident r;
+    if (resident_of(p, sh, gated, true, &r))
+    {
+        NormArgs s = slice_args(a, r);
+        s.channel_part = params ? static_cast<float2*>(io->workspace) : nullptr;
+        s.param_parts = p->batch;
+        ADOP_TRY(launch({"k_norm_grad_resident", kNormGradResident, r.threads, r.k, dim3((unsigned)r.k, (unsigned)p->batch << r.slices), r.smem, false}, p, sh,
+                        gated, s, st));
+        if (!params) return ADOP_OK;
+        return launch({"k_norm_grad_params", kNormGradParams, kNormGradThreads, 1, dim3((unsigned)((a.C + kParamChannels - 1) / kParamChannels)),
+                       sizeof(double) * 2 * kNormGradThreads, true}, p, sh, gated, s, st);
+    }
     int threads;
     threads_of(a.P, kNormGradThreads, &a.R, &threads);
-    a.lanes = lanes_for(a.Cg);
     const Share share = share_of(p, gated, true);
-    const int most = share.chunks < a.rows ? share.chunks : a.rows, k = cluster_of(most), chunks = most / k * k;
-    a.clusters = chunks / k;
-    const bool params = io->grad_weight || io->grad_bias;
-    a.group_part = static_cast<double2*>(io->workspace);
-    a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.clusters)) : nullptr;
-    a.param_parts = p->batch * a.clusters;
-    const size_t smem_sums = sizeof(double2) * a.G + sizeof(float) * (2 * (size_t)a.C + 2 * (size_t)a.P * sh.V) + sums_scratch(sh, 1, a.R, threads);
-    size_t smem_apply = apply_smem(a.G, threads);
+    finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
+    a.group_part = static_cast<float2*>(io->workspace);
+    a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.chunks)) : nullptr;
+    a.param_parts = p->batch * a.chunks;
+    const size_t smem_sums = sizeof(float2) * a.G + sizeof(float) * 4 * (size_t)a.C + sums_scratch(sh, 1, a.R, threads);
+    size_t smem_apply = apply_smem(a);
+    const int es = element_size(p->type);
     if (params && smem_apply < sizeof(double) * 2 * threads) smem_apply = sizeof(double) * 2 * threads;
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
     {
         const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
         // the parameters' gradients need the sums of all images: blocks of the last launch add them up
-        a.param_blocks = params && a.image0 + share.images >= p->batch ? (a.C + 31) / 32 : 0;
-        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, k, dim3((unsigned)chunks, n), smem_sums, a.image0 > 0}, p, sh, gated, a, st));
-        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, 1, dim3((unsigned)(chunks + a.param_blocks), n), smem_apply, true}, p, sh, gated, a, st));
+        a.param_blocks = params && a.image0 + share.images >= p->batch ? (a.C + kParamChannels - 1) / kParamChannels : 0;
+        a.vectors = (int)align16(smem_sums);
+        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_sums, sh, es, threads, gated, true),
+                         a.image0 > 0}, p, sh, gated, a, st));
+        a.vectors = (int)align16(smem_apply);
+        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, 1, dim3((unsigned)(a.chunks + a.param_blocks), n),
+                         stream_smem(smem_apply, sh, es, threads, gated, true), true}, p, sh, gated, a, st));
     }
     return ADOP_OK;
 }
@@ -337,13 +439,14 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
 namespace {
 adop_status gate_launch(const adop_norm_params* p, const Shape& sh, NormArgs& a, bool backward, cudaStream_t st)
 {
-    const int most = backward ? kNormGradThreads : kNormThreads;
+    const int most = backward ? kGateGradThreads : kGateThreads;
     int threads;
     threads_of(a.P, most, &a.R, &threads);
     const int64_t worth = (p->pixels * p->channels * element_size(p->type) + kMinChunk - 1) / kMinChunk;
-    int64_t chunks = ((int64_t)sm_count() * (backward ? kNormGradBlocks : kNormBlocks) + p->batch - 1) / p->batch;
+    int64_t chunks = ((int64_t)sm_count() * kGateBlocks + p->batch - 1) / p->batch;
     if (chunks > worth) chunks = worth;
     if (chunks > a.rows) chunks = a.rows;
+    finish(&a, threads, (int)chunks);
     return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, 1, dim3((unsigned)chunks, (unsigned)p->batch), 0, false}, p, sh,
                   true, a, st);
 }

@@ -23,32 +23,50 @@ namespace norm {
 namespace cg = cooperative_groups;
 
 // ---- vectors ------------------------------------------------------------------------------------------------------------
+// VEC values of a vector in 32 bits, in pairs: sm_100 adds, multiplies and fuses two at a time (one instruction a pair). With one
+// element the second of its pair is computed along and dropped.
+template <int VEC> struct alignas(VEC > 2 ? 16 : 8) Lanes
+{
+    static constexpr int N = (VEC + 1) / 2;
+    float2 p[N];
+    __device__ __forceinline__ float get(int j) const { return j & 1 ? p[j / 2].y : p[j / 2].x; }
+    __device__ __forceinline__ void set(int j, float v)
+    {
+        if (j & 1) p[j / 2].y = v;
+        else p[j / 2].x = v;
+    }
+    __device__ __forceinline__ void fill(float v)
+    {
+#pragma unroll
+        for (int k = 0; k < N; ++k) p[k] = make_float2(v, v);
+    }
+};
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
 template <int BYTES> struct Word;
 template <> struct Word<16> { using type = uint4; };
 template <> struct Word<8> { using type = uint2; };
 template <> struct Word<4> { using type = unsigned; };
 template <> struct Word<2> { using type = unsigned short; };
 
-template <typename T> __device__ __forceinline__ void unpack2(unsigned w, float& a, float& b);
-template <> __device__ __forceinline__ void unpack2<__nv_bfloat16>(unsigned w, float& a, float& b)
+template <typename T> __device__ __forceinline__ float2 unpack2(unsigned w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned w)
 {
-    a = __uint_as_float(w << 16);
-    b = __uint_as_float(w & 0xffff0000u);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <> __device__ __forceinline__ void unpack2<__half>(unsigned w, float& a, float& b)
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <typename T> __device__ __forceinline__ unsigned pack2(float2 v);
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float2 v)
 {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    a = f.x; b = f.y;
-}
-template <typename T> __device__ __forceinline__ unsigned pack2(float a, float b);
-template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float a, float b)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
     return *reinterpret_cast<const unsigned*>(&h);
 }
-template <> __device__ __forceinline__ unsigned pack2<__half>(float a, float b)
+template <> __device__ __forceinline__ unsigned pack2<__half>(float2 v)
 {
-    const __half2 h = __floats2half2_rn(a, b);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
     return *reinterpret_cast<const unsigned*>(&h);
 }
 template <typename T> __device__ __forceinline__ float to_float(T v);
@@ -66,33 +84,35 @@ template <typename T, int VEC> struct Vec
     static constexpr int kBytes = VEC * (int)sizeof(T);
     using W = typename Word<kBytes>::type;
     static __device__ __forceinline__ W load(const T* p) { return __ldg(reinterpret_cast<const W*>(p)); }
-    static __device__ __forceinline__ void unpack(const W& w, float (&v)[VEC])
+    static __device__ __forceinline__ Lanes<VEC> unpack(const W& w)
     {
-        if constexpr (VEC == 1) v[0] = to_float<T>(*reinterpret_cast<const T*>(&w));
+        Lanes<VEC> v;
+        if constexpr (VEC == 1) v.p[0] = pair(to_float<T>(*reinterpret_cast<const T*>(&w)));
         else
         {
             const unsigned* u = reinterpret_cast<const unsigned*>(&w);
 #pragma unroll
-            for (int k = 0; k < kBytes / 4; ++k)
+            for (int k = 0; k < VEC / 2; ++k)
             {
-                if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(u[k]);
-                else unpack2<T>(u[k], v[2 * k], v[2 * k + 1]);
+                if constexpr (sizeof(T) == 4) v.p[k] = make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
+                else v.p[k] = unpack2<T>(u[k]);
             }
         }
+        return v;
     }
     // rounded once, to nearest even
-    static __device__ __forceinline__ void store(T* p, const float (&v)[VEC])
+    static __device__ __forceinline__ void store(T* p, const Lanes<VEC>& v)
     {
-        if constexpr (VEC == 1) *p = from_float<T>(v[0]);
+        if constexpr (VEC == 1) *p = from_float<T>(v.p[0].x);
         else
         {
             W w;
             unsigned* u = reinterpret_cast<unsigned*>(&w);
 #pragma unroll
-            for (int k = 0; k < kBytes / 4; ++k)
+            for (int k = 0; k < VEC / 2; ++k)
             {
-                if constexpr (sizeof(T) == 4) u[k] = __float_as_uint(v[k]);
-                else u[k] = pack2<T>(v[2 * k], v[2 * k + 1]);
+                if constexpr (sizeof(T) == 4) { u[2 * k] = __float_as_uint(v.p[k].x); u[2 * k + 1] = __float_as_uint(v.p[k].y); }
+                else u[k] = pack2<T>(v.p[k]);
             }
             *reinterpret_cast<W*>(p) = w;
         }
@@ -105,6 +125,15 @@ __device__ __forceinline__ float load_param(const void* p, int type, int i)
     if (type == ADOP_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
+// weight and bias of the channels from c0 on as to[C] and to[C] behind it, 1 and 0 where there are none; a barrier follows
+__device__ __forceinline__ void stage_params(const NormArgs& a, int c0, float* to)
+{
+    for (int c = threadIdx.x; c < a.C; c += blockDim.x)
+    {
+        to[c] = a.weight ? load_param(a.weight, a.param_type, c0 + c) : 1.f;
+        to[a.C + c] = a.bias ? load_param(a.bias, a.param_type, c0 + c) : 0.f;
+    }
+}
 __device__ __forceinline__ void store_param(void* p, int type, int i, float v)
 {
     if (type == ADOP_TYPE_F32) static_cast<float*>(p)[i] = v;
@@ -113,652 +142,809 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v)
 }
 
 // ---- activations --------------------------------------------------------------------------------------------------------
-// sigmoid s and 1 - s, both to a few units of the last place: from e = exp(-|v|), which never overflows
-__device__ __forceinline__ void sigmoid_pair(float v, float& s, float& ns)
+constexpr float kLog2e = 1.4426950408889634f;
+// powers of two and reciprocals of the special-function unit (2 ulp; results below the smallest normal number become 0)
+__device__ __forceinline__ float ex2(float v)
 {
-    const float e = __expf(-fabsf(v));
-    const float t = __fdividef(1.f, 1.f + e);
-    const float et = e * t;
-    s = v >= 0.f ? t : et;
-    ns = v >= 0.f ? et : t;
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
-__device__ __forceinline__ float sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-// exp(v) - 1 for v <= 0. For 16-bit images: near zero, where exp(v) - 1 loses digits, its Taylor series (the first term left
-// out is v^6 / 720, relative to v below 2^-24 for |v| < 1/8).
-template <typename T> __device__ __forceinline__ float expm1_neg(float v, float e)
+__device__ __forceinline__ float rcp(float v)
 {
-    if constexpr (sizeof(T) == 4) return expm1f(v);
-    const float series = v * fmaf(v, fmaf(v, fmaf(v, fmaf(v, 1.f / 120.f, 1.f / 24.f), 1.f / 6.f), 0.5f), 1.f);
-    return v > -0.125f ? series : e - 1.f;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float2 exp2v(float2 v) { return make_float2(ex2(v.x), ex2(v.y)); }
+__device__ __forceinline__ float2 rcp2(float2 v) { return make_float2(rcp(v.x), rcp(v.y)); }
+__device__ __forceinline__ float2 sigmoid(float2 v) { return rcp2(add(exp2v(mul(v, pair(-kLog2e))), pair(1.f))); }
+// sigmoid s and 1 - s, both to a few units of the last place: from e = exp(-|v|), which never overflows
+__device__ __forceinline__ void sigmoid_pair(float2 v, float2& s, float2& ns)
+{
+    const float2 e = exp2v(mul(make_float2(fabsf(v.x), fabsf(v.y)), pair(-kLog2e)));
+    const float2 t = rcp2(add(e, pair(1.f))), et = mul(e, t);
+    s = make_float2(v.x >= 0.f ? t.x : et.x, v.y >= 0.f ? t.y : et.y);
+    ns = make_float2(v.x >= 0.f ? et.x : t.x, v.y >= 0.f ? et.y : t.y);
+}
+// v > 0 ? v : exp(v) - 1, with e = exp(v). Near zero, where e - 1 loses digits, the Taylor series: for 16-bit images four terms above
+// -1/16 (the fifth is below 2^-22 of the sum there), for 32 bits eight above -1/2 (the ninth is below 2^-26).
+template <typename T> __device__ __forceinline__ float2 elu_value(float2 v, float2 e)
+{
+    constexpr bool kWide = sizeof(T) == 4;
+    constexpr float kFrom = kWide ? -0.5f : -0.0625f;
+    float2 q = pair(1.f / 24.f);
+    if (kWide)
+    {
+        q = fma2(v, pair(1.f / 40320.f), pair(1.f / 5040.f));
+        q = fma2(v, q, pair(1.f / 720.f));
+        q = fma2(v, q, pair(1.f / 120.f));
+        q = fma2(v, q, pair(1.f / 24.f));
+    }
+    q = fma2(v, q, pair(1.f / 6.f));
+    q = fma2(v, q, pair(0.5f));
+    q = fma2(v, q, pair(1.f));
+    q = mul(v, q);
+    const float2 m = add(e, pair(-1.f));
+    return make_float2(v.x > 0.f ? v.x : (v.x > kFrom ? q.x : m.x), v.y > 0.f ? v.y : (v.y > kFrom ? q.y : m.y));
 }
 // ACT = one of ADOP_ACTIVATION_* (rt ignored) or 4: rt says which, the same for all threads
-template <typename T, int ACT> __device__ __forceinline__ float act_value(float v, int rt)
+template <typename T, int ACT> __device__ __forceinline__ float2 act_value(float2 v, int rt)
 {
     const int a = ACT < 4 ? ACT : rt;
-    if (a == ADOP_ACTIVATION_RELU) return v < 0.f ? 0.f : v;  // a NaN stays one
-    if (a == ADOP_ACTIVATION_ELU) return v > 0.f ? v : expm1_neg<T>(v, __expf(v));
-    if (a == ADOP_ACTIVATION_SILU) return v * sigmoid(v);
+    if (a == ADOP_ACTIVATION_RELU) return make_float2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);  // a NaN stays one
+    if (a == ADOP_ACTIVATION_ELU) return elu_value<T>(v, exp2v(mul(v, pair(kLog2e))));
+    if (a == ADOP_ACTIVATION_SILU) return mul(v, sigmoid(v));
     return v;
 }
 // d act'(v)
-template <typename T, int ACT> __device__ __forceinline__ float act_grad(float v, float d, int rt)
+template <typename T, int ACT> __device__ __forceinline__ float2 act_grad(float2 v, float2 d, int rt)
 {
     const int a = ACT < 4 ? ACT : rt;
-    if (a == ADOP_ACTIVATION_RELU) return v <= 0.f ? 0.f : d;
-    if (a == ADOP_ACTIVATION_ELU) return v > 0.f ? d : d * __expf(v);
+    if (a == ADOP_ACTIVATION_RELU) return make_float2(v.x <= 0.f ? 0.f : d.x, v.y <= 0.f ? 0.f : d.y);
+    if (a == ADOP_ACTIVATION_ELU)
+    {
+        const float2 e = exp2v(mul(v, pair(kLog2e)));
+        return make_float2(v.x > 0.f ? d.x : d.x * e.x, v.y > 0.f ? d.y : d.y * e.y);
+    }
     if (a == ADOP_ACTIVATION_SILU)
     {
-        float s, ns;
+        float2 s, ns;
         sigmoid_pair(v, s, ns);
-        return d * (s * fmaf(v, ns, 1.f));
+        return mul(d, mul(s, fma2(v, ns, pair(1.f))));
     }
     return d;
 }
 // act(f) and act'(f) together
-template <typename T, int ACT> __device__ __forceinline__ void act_both(float v, float& value, float& slope, int rt)
+template <typename T, int ACT> __device__ __forceinline__ void act_both(float2 v, float2& value, float2& slope, int rt)
 {
     const int a = ACT < 4 ? ACT : rt;
-    value = v; slope = 1.f;
-    if (a == ADOP_ACTIVATION_RELU) { value = v < 0.f ? 0.f : v; slope = v <= 0.f ? 0.f : 1.f; }
+    value = v; slope = pair(1.f);
+    if (a == ADOP_ACTIVATION_RELU)
+    {
+        value = make_float2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y);
+        slope = make_float2(v.x <= 0.f ? 0.f : 1.f, v.y <= 0.f ? 0.f : 1.f);
+    }
     if (a == ADOP_ACTIVATION_ELU)
     {
-        const float e = __expf(v);
-        value = v > 0.f ? v : expm1_neg<T>(v, e);
-        slope = v > 0.f ? 1.f : e;
+        const float2 e = exp2v(mul(v, pair(kLog2e)));
+        value = elu_value<T>(v, e);
+        slope = make_float2(v.x > 0.f ? 1.f : e.x, v.y > 0.f ? 1.f : e.y);
     }
     if (a == ADOP_ACTIVATION_SILU)
     {
-        float s, ns;
+        float2 s, ns;
         sigmoid_pair(v, s, ns);
-        value = v * s;
-        slope = s * fmaf(v, ns, 1.f);
+        value = mul(v, s);
+        slope = mul(s, fma2(v, ns, pair(1.f)));
     }
 }
 
+// i / d for i, d up to 4096 (quotient off an integer by 1 / 2d at least, the product by 2^-22 of it), inv = 1 / d
+__device__ __forceinline__ int quotient(int i, float inv) { return (int)(((float)i + 0.5f) * inv); }
+
 // ---- where a thread works -----------------------------------------------------------------------------------------------
+// A thread's vector of the row and its first row of the block's chunk; the rows after it are R apart.
 struct Place
 {
-    int ph, r0;   // vector of the row, first row in the block's chunk
+    int ph, r0;
     bool active;
+    __device__ __forceinline__ Place(const NormArgs& a, int ph0)
+    {
+        const int t = threadIdx.x;
+        if (a.R == 1) { ph = ph0 + t; r0 = 0; }
+        else { r0 = quotient(t, a.inv_P); ph = t - r0 * a.P; }
+        active = ph < a.P && r0 < a.R;
+    }
+    // how many rows of [begin, end) are the thread's
+    __device__ __forceinline__ int count(const NormArgs& a, int begin, int end) const
+    {
+        const int left = end - begin - r0;
+        return left <= 0 ? 0 : (left - 1) / a.R + 1;
+    }
 };
-template <typename T> __device__ __forceinline__ const T* at(const NormImage& im, int b, int slice_c, int64_t row, int ph, int vec)
+// The vectors of a tensor that a thread comes by: `step` elements apart, forwards from the chunk's first row or backwards from its last.
+template <typename T> struct Walk
 {
-    return static_cast<const T*>(im.p) + (int64_t)b * im.image + slice_c + row * im.row + (int64_t)ph * vec;
+    T* p;
+    int64_t step;
+    __device__ __forceinline__ Walk(const NormImage& im, int b, int c0, const Place& pl, int R, int vec, int begin, int end, bool backwards)
+    {
+        const int64_t row = backwards ? (int64_t)end - 1 - pl.r0 : (int64_t)begin + pl.r0;
+        p = static_cast<T*>(const_cast<void*>(im.p)) + (int64_t)b * im.image + c0 + row * im.row + (int64_t)pl.ph * vec;
+        step = (backwards ? -im.row : im.row) * R;
+    }
+    __device__ __forceinline__ T* at(int k) const { return p + k * step; }
+    __device__ __forceinline__ void on(int k) { p += k * step; }
+};
+// U loads are under way before the first is used
+template <int U, class Load, class Use, class Next> __device__ __forceinline__ void batches(int n, Load load, Use use, Next next)
+{
+    int i = 0;
+    for (; i + U <= n; i += U)
+    {
+        decltype(load(0)) in[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) in[k] = load(k);
+#pragma unroll
+        for (int k = 0; k < U; ++k) use(k, in[k]);
+        next(U);
+    }
+    if (U > 1 && i < n)
+    {
+        decltype(load(0)) in[U];
+#pragma unroll
+        for (int k = 0; k < U - 1; ++k)
+            if (i + k < n) in[k] = load(k);
+#pragma unroll
+        for (int k = 0; k < U - 1; ++k)
+            if (i + k < n) use(k, in[k]);
+    }
 }
-template <typename T> __device__ __forceinline__ T* at_out(const NormImage& im, int b, int slice_c, int64_t row, int ph, int vec)
+// rows [begin, end) of a part of the image: of the parts, the first chunk_more have a row more than the others
+__device__ __forceinline__ void chunk_of(const NormArgs& a, int part, int& begin, int& end)
 {
-    return const_cast<T*>(at<T>(im, b, slice_c, row, ph, vec));
+    begin = part * a.chunk_rows + min(part, a.chunk_more);
+    end = begin + a.chunk_rows + (part < a.chunk_more ? 1 : 0);
 }
-__device__ __forceinline__ void chunk_of(int rows, int part, int parts, int& begin, int& end)
+// f(j, c, g) for the channels c and groups g of a thread's vector (a row of several pixels goes through the channels again)
+template <int VEC, class F> __device__ __forceinline__ void for_channels(const NormArgs& a, int ph, F f)
 {
-    begin = (int)((int64_t)rows * part / parts);
-    end = (int)((int64_t)rows * (part + 1) / parts);
+    int c = ph * VEC;
+    while (c >= a.C) c -= a.C;
+    int g = quotient(c, a.inv_Cg), r = c - g * a.Cg;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+    {
+        f(j, c, g);
+        ++c;
+        if (++r == a.Cg) { r = 0; ++g; }
+        if (c == a.C) c = g = 0;
+    }
 }
 // A kernel that was launched while the one before it may still run waits here for that one's results; every kernel that may
 // be launched so waits before it ends, so that whoever waits for it also has all that came before.
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-template <typename T, int VEC, bool GATED> struct Loaded
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from)
 {
-    typename Vec<T, VEC>::W x, g;
+    const unsigned s = (unsigned)__cvta_generic_to_shared(to);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(s), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+template <typename T, int VEC> struct Input
+{
+    typename Vec<T, VEC>::W x, g, dy;
+};
+// The vectors of x, of the gate and of dy that a thread comes by in a chunk. Copies into slots of its own in shared memory run D vectors
+// ahead, the first D of them from start() on, which may stand far in front of run(): what a block does before its loop, and its waits,
+// cost no bandwidth then. 64 to 98 KB are under way on an SM; registers hold one vector. Vectors of one element have no such copies:
+// there U loads are under way before the first is used.
+template <typename T, int VEC, bool GATED, bool GRAD> struct Stream
+{
+    static constexpr int kTensors = 1 + (GATED ? 1 : 0) + (GRAD ? 1 : 0);
+    static constexpr int D = stream_depth(GATED, GRAD);
+    using V = Vec<T, VEC>;
+    using W = typename V::W;
+    using In = Input<T, VEC>;
+    Walk<T> x, g, d;
+    int n;
+    W* slots;
+    __device__ __forceinline__ Stream(const NormArgs& a, int b, const Place& pl, int begin, int end, bool backwards, void* shared)
+        : x(a.x, b, 0, pl, a.R, VEC, begin, end, backwards), g(a.gate, b, 0, pl, a.R, VEC, begin, end, backwards),
+          d(a.dy, b, 0, pl, a.R, VEC, begin, end, backwards), n(pl.active ? pl.count(a, begin, end) : 0),
+          slots(reinterpret_cast<W*>(static_cast<char*>(shared) + a.vectors) + threadIdx.x)
+    {
+    }
+    __device__ __forceinline__ W* slot(int i) const { return slots + (i & (D - 1)) * kTensors * blockDim.x; }
+    __device__ __forceinline__ void copy(int i)
+    {
+        W* s = slot(i);
+        copy_async<V::kBytes>(s, x.p);
+        x.on(1);
+        if constexpr (GATED)
+        {
+            copy_async<V::kBytes>(s + blockDim.x, g.p);
+            g.on(1);
+        }
+        if constexpr (GRAD)
+        {
+            copy_async<V::kBytes>(s + (kTensors - 1) * blockDim.x, d.p);
+            d.on(1);
+        }
+    }
+    __device__ __forceinline__ void start()
+    {
+        if constexpr (VEC > 1)
+#pragma unroll
+            for (int i = 0; i < D; ++i)
+            {
+                if (i < n) copy(i);
+                copies_commit();
+            }
+    }
+    template <class Use> __device__ __forceinline__ void run(Use use)
+    {
+        if constexpr (VEC > 1)
+        {
+            for (int i = 0; i < n; ++i)
+            {
+                copies_wait<D - 1>();
+                const W* s = slot(i);
+                In in;
+                in.x = s[0];
+                if constexpr (GATED) in.g = s[blockDim.x];
+                if constexpr (GRAD) in.dy = s[(kTensors - 1) * blockDim.x];
+                use(in);
+                if (i + D < n) copy(i + D);
+                copies_commit();
+            }
+        }
+        else
+        {
+            constexpr int U = 4;
+            for (int i = 0; i < n; i += U)
+            {
+                In in[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (i + k < n)
+                    {
+                        in[k].x = V::load(x.at(k));
+                        if constexpr (GATED) in[k].g = V::load(g.at(k));
+                        if constexpr (GRAD) in[k].dy = V::load(d.at(k));
+                    }
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (i + k < n) use(in[k]);
+                x.on(U); g.on(U); d.on(U);
+            }
+        }
+    }
 };
 // u of a vector
-template <typename T, int VEC, bool GATED, int ACT>
-__device__ __forceinline__ void value_of(const Loaded<T, VEC, GATED>& in, float (&u)[VEC], int rt)
+template <typename T, int VEC, bool GATED, int ACT> __device__ __forceinline__ Lanes<VEC> value_of(const Input<T, VEC>& in, int rt)
 {
-    Vec<T, VEC>::unpack(in.x, u);
+    Lanes<VEC> u = Vec<T, VEC>::unpack(in.x);
     if constexpr (GATED)
     {
-        float g[VEC];
-        Vec<T, VEC>::unpack(in.g, g);
+        const Lanes<VEC> g = Vec<T, VEC>::unpack(in.g);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) u[j] = act_value<T, ACT>(u[j], rt) * sigmoid(g[j]);
+        for (int k = 0; k < Lanes<VEC>::N; ++k) u.p[k] = mul(act_value<T, ACT>(u.p[k], rt), sigmoid(g.p[k]));
     }
+    return u;
 }
 
 // ---- sums of a block ----------------------------------------------------------------------------------------------------
-// v[k][j]: two sums of each of a thread's channels. Runs of m channels are added up first. tot[(k * (VEC / m) + j / m) * P + ph]
-// gets the sums over the rows of the block; buf is scratch of 2 (VEC / m) rows P + blockDim floats. Fixed order: the same
-// bits on every run.
-template <int VEC>
-__device__ __forceinline__ void block_sums(float (&v)[2][VEC], int m, const NormArgs& a, const Place& at, float* tot, float* buf)
+// v[k]: two sums of each of a thread's channels. Runs of m channels are added up first, then the lanes of a warp that have the same
+// channels; what is left goes to buf[(slot * rows + row) * P + ph], slot = k (VEC / m) + j / m. Returns rows. The caller waits at a
+// barrier and adds the rows up, in a fixed order: the same bits on every run. In all 2 (VEC / m) rows P floats.
+__device__ __forceinline__ int sum_rows(const NormArgs& a) { return 32 % a.P == 0 ? (int)blockDim.x >> 5 : a.R; }
+template <int VEC, int STEP>
+__device__ __forceinline__ void put_sums(Lanes<VEC> (&v)[2], const NormArgs& a, const Place& pl, float* buf)
 {
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-    {
-        if (VEC > 1 && m > 1)
-#pragma unroll
-            for (int j = 0; j + 1 < VEC; j += 2) v[k][j] += v[k][j + 1];
-        if (VEC > 2 && m > 2)
-#pragma unroll
-            for (int j = 0; j + 2 < VEC; j += 4) v[k][j] += v[k][j + 2];
-        if (VEC > 4 && m > 4) v[k][0] += v[k][VEC / 2];
-    }
-    const int sh = __ffs(m) - 1, per = VEC >> sh, P = a.P, t = threadIdx.x, T = blockDim.x;
-    if (a.R == 1)
-    {
-        if (at.active)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if ((j & (m - 1)) == 0) tot[(k * per + (j >> sh)) * P + at.ph] = v[k][j];
-        return;
-    }
-    int rows = a.R, row = at.r0;
-    bool writer = at.active;
+    constexpr int per = VEC / STEP;
+    const int P = a.P, rows = sum_rows(a);
+    int row = pl.r0;
+    bool writer = pl.active;
     if (32 % P == 0)
     {
-        // the lanes of a warp that have the same channels
         for (int o = 16; o >= P; o >>= 1)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    if ((j & (m - 1)) == 0) v[k][j] += __shfl_xor_sync(0xffffffffu, v[k][j], o);
-        rows = T >> 5; row = t >> 5;
-        writer = (t & 31) < P;
+                for (int j = 0; j < VEC; j += STEP) v[k].set(j, v[k].get(j) + __shfl_xor_sync(0xffffffffu, v[k].get(j), o));
+        row = threadIdx.x >> 5;
+        writer = (threadIdx.x & 31) < P;
     }
     if (writer)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j)
-                if ((j & (m - 1)) == 0) buf[((k * per + (j >> sh)) * rows + row) * P + at.ph] = v[k][j];
-    __syncthreads();
-    const int items = 2 * per * P;
-    const int parts = min(rows, max(1, T / items));
-    if (parts == 1)
-    {
-        for (int i = t; i < items; i += T)
+            for (int j = 0; j < VEC; j += STEP) buf[((k * per + j / STEP) * rows + row) * P + pl.ph] = v[k].get(j);
+}
+template <int VEC>
+__device__ __forceinline__ void block_sums(Lanes<VEC> (&v)[2], int m, const NormArgs& a, const Place& pl, float* buf)
+{
+    if (VEC > 1 && m > 1)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j + 1 < VEC; j += 2) v[k].p[j / 2].x += v[k].p[j / 2].y;
+    if (VEC > 2 && m > 2)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j + 2 < VEC; j += 4) v[k].p[j / 2].x += v[k].p[j / 2 + 1].x;
+    if constexpr (VEC > 4)
+        if (m == 8)
         {
-            const float* col = buf + (i / P) * rows * P + i % P;
-            float s = 0.f;
-#pragma unroll 4
-            for (int r = 0; r < rows; ++r) s += col[r * P];
-            tot[i] = s;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) v[k].p[0].x += v[k].p[2].x;
+            return put_sums<VEC, 8>(v, a, pl, buf);
         }
-        return;
-    }
-    float* tmp = buf + items * rows;
-    if (t < items * parts)
+    if constexpr (VEC > 2)
+        if (m == 4) return put_sums<VEC, 4>(v, a, pl, buf);
+    if constexpr (VEC > 1)
+        if (m == 2) return put_sums<VEC, 2>(v, a, pl, buf);
+    put_sums<VEC, 1>(v, a, pl, buf);
+}
+
+// The block's sums of u and u^2 of a group in 64 bits, for f(g, sums), from the slots' sums of u - pivot and its square over `n` rows
+// of the image. The pivots are values of the data themselves, so the squares cancel by the number of values at most.
+template <int VEC, class F>
+__device__ __forceinline__ void group_sums(const NormArgs& a, int n, const float* buf, const float* pivot, F f)
+{
+    const int sh = __ffs(a.m) - 1, per = VEC >> sh, run = a.Cg >> sh, slots = run * a.ppr, rows = sum_rows(a), second = per * rows * a.P;
+    const int lanes = 1 << a.lanes, row_lanes = 1 << a.row_lanes, want = ((a.G << a.lanes) + 31) & ~31;
+    const double cnt = (double)n * (double)a.m;
+    for (int idx = threadIdx.x; idx < want; idx += blockDim.x)
     {
-        const int i = t % items;
-        const float* col = buf + (i / P) * rows * P + i % P;
-        float s = 0.f;
-        for (int r = t / items; r < rows; r += parts) s += col[r * P];
-        tmp[t] = s;
-    }
-    __syncthreads();
-    if (t < items)
-    {
-        float s = 0.f;
-        for (int q = 0; q < parts; ++q) s += tmp[q * items + t];
-        tot[t] = s;
+        const int g = idx >> a.lanes, lane = idx & (lanes - 1), row = lane & (row_lanes - 1);
+        double s = 0.0, q = 0.0;
+        // a group's lanes: row_lanes for a slot's rows, so many slots at a time; the same number of turns for all of them
+        for (int slot0 = 0; slot0 < slots; slot0 += lanes >> a.row_lanes)
+        {
+            const int slot = slot0 + (lane >> a.row_lanes);
+            const bool here = g < a.G && slot < slots;
+            float ds = 0.f, dq = 0.f;
+            double piv = 0.0;
+            if (here)
+            {
+                int i = slot, e = g * a.Cg;
+                while (i >= run) { i -= run; e += a.C; }
+                e += i << sh;
+                const int jj = (e % VEC) >> sh, p = e / VEC;
+                piv = (double)pivot[jj * a.P + p];
+                const float* col = buf + jj * rows * a.P + p;
+                for (int r = row; r < rows; r += row_lanes) { ds += col[r * a.P]; dq += col[second + r * a.P]; }
+            }
+            for (int o = row_lanes >> 1; o > 0; o >>= 1)
+            {
+                ds += __shfl_xor_sync(0xffffffffu, ds, o);
+                dq += __shfl_xor_sync(0xffffffffu, dq, o);
+            }
+            if (here)
+            {
+                const double d = (double)ds;
+                s += fma(cnt, piv, d);
+                q += fma(piv, fma(cnt, piv, 2.0 * d), (double)dq);
+            }
+        }
+        for (int o = lanes >> 1; o >= row_lanes; o >>= 1)
+        {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            q += __shfl_xor_sync(0xffffffffu, q, o);
+        }
+        if (g < a.G && lane == 0) f(g, make_double2(s, q));
     }
 }
 
-// The group's sums of u and u^2 in 64 bits from the slots' sums of u - pivot and its square over `rows` rows. The pivots are
-// values of the data themselves, so the squares cancel by the number of values at most.
-template <int VEC>
-__device__ __forceinline__ void group_sums(const NormArgs& a, int rows, const float* tot, const float* pivot, double2* out)
+// f(g, sums) for the groups of an image from the partial sums [G, chunks] of its chunks, part(k, v) = what partial sum k stands for in
+// 64 bits; by 2^a.gather threads a group. The caller waits at a barrier.
+template <class Part, class F>
+__device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part part, F f)
 {
-    const int per = VEC / a.m, run = a.Cg / a.m, n = run * a.ppr, lanes = a.lanes, T = blockDim.x;
-    const int want = (a.G * lanes + 31) & ~31;
-    const double cnt = (double)rows * a.m;
-    for (int idx = threadIdx.x; idx < want; idx += T)
+    const float2* __restrict__ from = a.group_part + (size_t)b * a.chunks * a.G;
+    const int lanes = 1 << a.gather, want = ((a.G << a.gather) + 31) & ~31;
+    for (int idx = threadIdx.x; idx < want; idx += blockDim.x)
     {
-        const int g = idx / lanes, lane = idx & (lanes - 1);
+        const int g = idx >> a.gather, lane = idx & (lanes - 1);
+        double2 sum = make_double2(0.0, 0.0);
+        if (g < a.G)
+#pragma unroll 8
+            for (int k = lane; k < a.chunks; k += lanes)
+            {
+                const double2 v = part(k, __ldcg(from + (size_t)g * a.chunks + k));
+                sum.x += v.x; sum.y += v.y;
+            }
+        for (int o = lanes >> 1; o > 0; o >>= 1)
+        {
+            sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
+            sum.y += __shfl_xor_sync(0xffffffffu, sum.y, o);
+        }
+        if (g < a.G && lane == 0) f(g, sum);
+    }
+}
+// element g of a [G] array of every block of the cluster, added up
+__device__ __forceinline__ double2 cluster_sum(cg::cluster_group& cluster, double2* own, int g)
+{
+    const int k = (int)cluster.num_blocks();
+    if (k == 1) return own[g];
+    double2 s = make_double2(0.0, 0.0);
+    for (int o = 0; o < k; ++o)
+    {
+        const double2 v = cluster.map_shared_rank(own, o)[g];
+        s.x += v.x; s.y += v.y;
+    }
+    return s;
+}
+__device__ __forceinline__ float2 mean_rstd(double2 sums, double inv_n, float eps)
+{
+    const double mean = sums.x * inv_n;
+    double var = fma(-mean, mean, sums.y * inv_n);
+    if (var < 0.0) var = 0.0;  // a NaN stays one
+    return make_float2((float)mean, (float)rsqrt(var + (double)eps));
+}
+
+// ---- coefficients of a thread's channels ----------------------------------------------------------------------------------
+// (u - mean) scale + b is one fused u scale + (b - mean scale): what that rounds, 2^-25 of mean scale, is what the mean's own
+// rounding costs too, and a vector's channels need two registers each instead of three.
+template <int VEC> struct Forward
+{
+    Lanes<VEC> scale, shift;
+    __device__ __forceinline__ void set(const NormArgs& a, int ph, const float2* stat, const float* params)
+    {
+        scale.fill(0.f); shift.fill(0.f);
+        for_channels<VEC>(a, ph, [&](int j, int c, int g) {
+            const float2 s = stat[g];
+            const float k = s.y * params[c];
+            scale.set(j, k);
+            shift.set(j, fmaf(-s.x, k, params[a.C + c]));
+        });
+    }
+};
+template <typename T, int VEC, bool GATED, int ACT>
+__device__ __forceinline__ void normalise(Lanes<VEC>& u, const Forward<VEC>& f, int rt)
+{
+#pragma unroll
+    for (int k = 0; k < Lanes<VEC>::N; ++k)
+    {
+        const float2 z = fma2(u.p[k], f.scale.p[k], f.shift.p[k]);
+        u.p[k] = GATED ? z : act_value<T, ACT>(z, rt);
+    }
+}
+// one pivot for the channels that are added up together, the first of them; as its negative
+template <int VEC> __device__ __forceinline__ Lanes<VEC> pivot_of(const Lanes<VEC>& u, int m)
+{
+    Lanes<VEC> p;
+    p.fill(0.f);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) p.set(j, (j & (m - 1)) ? p.get(j - 1) : -u.get(j));
+    return p;
+}
+// A thread's sums are about its own first value: turned to that of the block's first row, which `shared` gets, n values a channel each.
+// One barrier.
+template <int VEC>
+__device__ __forceinline__ void common_pivot(Lanes<VEC> (&v)[2], const Lanes<VEC>& own, int n, const NormArgs& a, const Place& pl, float* shared)
+{
+    const int sh = __ffs(a.m) - 1;
+    if (pl.active && pl.r0 == 0)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if ((j & (a.m - 1)) == 0) shared[(j >> sh) * a.P + pl.ph] = -own.get(j);
+    __syncthreads();
+    if (n > 0 && pl.r0 > 0)
+    {
+        const float2 cnt = pair((float)n);
+#pragma unroll
+        for (int k = 0; k < Lanes<VEC>::N; ++k)
+        {
+            float2 d;
+            d.x = -own.p[k].x - shared[(2 * k >> sh) * a.P + pl.ph];
+            d.y = VEC > 1 ? -own.p[k].y - shared[((2 * k + 1) >> sh) * a.P + pl.ph] : d.x;
+            const float2 nd = mul(cnt, d);
+            v[1].p[k] = add(v[1].p[k], mul(d, add(add(v[0].p[k], v[0].p[k]), nd)));
+            v[0].p[k] = add(v[0].p[k], nd);
+        }
+    }
+}
+template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>& u, const Lanes<VEC>& pivot, Lanes<VEC> (&v)[2])
+{
+#pragma unroll
+    for (int k = 0; k < Lanes<VEC>::N; ++k)
+    {
+        const float2 d = add(u.p[k], pivot.p[k]);
+        v[0].p[k] = add(v[0].p[k], d);
+        v[1].p[k] = fma2(d, d, v[1].p[k]);
+    }
+}
+
+// ---- forward, images larger than a cluster's shared memory ------------------------------------------------------------------
+// Two launches, sums and what follows, a block on each SM for either. Both take less than half an SM and may start while the launch in
+// front of them runs: the next images' sums and these images' results share the SMs, and a launch has its first vectors when its turn
+// comes.
+// Shared memory: float pivots[P VEC / m] | block_sums' scratch | vectors
+template <typename T, int VEC, bool GATED, int ACT>
+__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const __grid_constant__ NormArgs a)
+{
+    extern __shared__ double2 smem[];
+    let_next_start();
+    const int b = a.image0 + blockIdx.y;
+    int begin, end;
+    chunk_of(a, blockIdx.x, begin, end);
+    float* shared = reinterpret_cast<float*>(smem);
+    float* buf = shared + a.P * (VEC / a.m);
+    for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
+    {
+        const Place pl(a, ph0);
+        Lanes<VEC> v[2], pivot;
+        v[0].fill(0.f); v[1].fill(0.f); pivot.fill(0.f);
+        Stream<T, VEC, GATED, false> in(a, b, pl, begin, end, false, smem);
+        in.start();
+        bool have = false;
+        in.run([&](const Input<T, VEC>& i) {
+            const Lanes<VEC> u = value_of<T, VEC, GATED, ACT>(i, a.act);
+            if (!have) pivot = pivot_of<VEC>(u, a.m);
+            have = true;
+            add_moments<VEC>(u, pivot, v);
+        });
+        common_pivot<VEC>(v, pivot, in.n, a, pl, shared);
+        block_sums<VEC>(v, a.m, a, pl, buf);
+    }
+    __syncthreads();
+    float2* out = a.group_part + (size_t)b * a.chunks * a.G + blockIdx.x;
+    const double inv_n = (int)blockIdx.x < a.chunk_more ? a.inv_long : a.inv_short;
+    group_sums<VEC>(a, end - begin, buf, shared, [&](int g, double2 sums) {
+        // the chunk's mean and sum of squares about it: 32 bits hold these
+        const double mean = sums.x * inv_n;
+        out[(size_t)g * a.chunks] = make_float2((float)mean, (float)fma(-mean, sums.x, sums.y));
+    });
+    wait_previous();
+}
+
+// Shared memory: float2 stat[G] | float params[2 C] | vectors
+template <typename T, int VEC, bool GATED, int ACT>
+__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_apply(const __grid_constant__ NormArgs a)
+{
+    extern __shared__ double2 smem[];
+    let_next_start();
+    const int T_ = blockDim.x, b = a.image0 + blockIdx.y;
+    int begin, end;
+    chunk_of(a, blockIdx.x, begin, end);
+    float2* stat = reinterpret_cast<float2*>(smem);
+    float* params = reinterpret_cast<float*>(stat + a.G);
+    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
+    {
+        const Place pl(a, ph0);
+        // from the end: what the sums read last is what the L2 still has
+        Stream<T, VEC, GATED, false> in(a, b, pl, begin, end, true, smem);
+        in.start();
+        if (ph0 == 0)
+        {
+            stage_params(a, 0, params);
+            wait_previous();
+            const double per_row = (double)(a.ppr * a.Cg);
+            gather_groups(
+                a, b,
+                [&](int k, float2 v) {
+                    const double mean = v.x, s = (double)(a.chunk_rows + (k < a.chunk_more ? 1 : 0)) * per_row * mean;
+                    return make_double2(s, fma(s, mean, (double)v.y));
+                },
+                [&](int g, double2 sums) {
+                    const float2 s = mean_rstd(sums, a.inv_n, a.eps);
+                    stat[g] = s;
+                    if (a.mean && blockIdx.x == 0)
+                    {
+                        a.mean[(size_t)b * a.G + g] = s.x;
+                        a.rstd[(size_t)b * a.G + g] = s.y;
+                    }
+                });
+            __syncthreads();
+        }
+        if (!pl.active) continue;
+        Forward<VEC> f;
+        f.set(a, pl.ph, stat, params);
+        Walk<T> y(a.y, b, 0, pl, a.R, VEC, begin, end, true);
+        in.run([&](const Input<T, VEC>& i) {
+            Lanes<VEC> u = value_of<T, VEC, GATED, ACT>(i, a.act);
+            normalise<T, VEC, GATED, ACT>(u, f, a.act);
+            Vec<T, VEC>::store(y.p, u);
+            y.on(1);
+        });
+    }
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------
+// uhat = u rstd + centre and z = uhat w + b of a vector
+template <int VEC> struct Saved
+{
+    Lanes<VEC> rstd, centre, w, bias;
+    __device__ __forceinline__ void set(const NormArgs& a, int ph, const float2* stat, const float* params)
+    {
+        rstd.fill(0.f); centre.fill(0.f); w.fill(0.f); bias.fill(0.f);
+        for_channels<VEC>(a, ph, [&](int j, int c, int g) {
+            const float2 s = stat[g];
+            rstd.set(j, s.y);
+            centre.set(j, -s.x * s.y);
+            w.set(j, params[c]);
+            bias.set(j, params[a.C + c]);
+        });
+    }
+};
+// mean and rstd of the image's groups from g0 on; a barrier follows
+__device__ __forceinline__ void stage_stats(const NormArgs& a, size_t g0, float2* to)
+{
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x) to[g] = make_float2(a.mean[g0 + g], a.rstd[g0 + g]);
+}
+template <typename T, int VEC, bool GATED, int ACT>
+__device__ __forceinline__ void add_grad_sums(const Input<T, VEC>& in, const Saved<VEC>& s, Lanes<VEC> (&v)[2], int rt)
+{
+    const Lanes<VEC> u = value_of<T, VEC, GATED, ACT>(in, rt), d = Vec<T, VEC>::unpack(in.dy);
+#pragma unroll
+    for (int k = 0; k < Lanes<VEC>::N; ++k)
+    {
+        const float2 uhat = fma2(u.p[k], s.rstd.p[k], s.centre.p[k]);
+        const float2 dz = GATED ? d.p[k] : act_grad<T, ACT>(fma2(uhat, s.w.p[k], s.bias.p[k]), d.p[k], rt);
+        v[0].p[k] = add(v[0].p[k], dz);
+        v[1].p[k] = fma2(dz, uhat, v[1].p[k]);
+    }
+}
+// z = u scale + shift, du = dz scale + u slope + offset, with scale = rstd w, slope = -rstd^2 c2, offset = -rstd c1 - mean slope
+template <int VEC> struct Backward
+{
+    Lanes<VEC> scale, shift, slope, offset;
+    __device__ __forceinline__ void set(const NormArgs& a, int ph, const float2* stat, const float2* c12, const float* params)
+    {
+        scale.fill(0.f); shift.fill(0.f); slope.fill(0.f); offset.fill(0.f);
+        for_channels<VEC>(a, ph, [&](int j, int c, int g) {
+            const float2 st = stat[g], c_ = c12[g];
+            const float r = st.y, mean = st.x, k = r * params[c], sl = -r * r * c_.y;
+            scale.set(j, k);
+            shift.set(j, fmaf(-mean, k, params[a.C + c]));
+            slope.set(j, sl);
+            offset.set(j, fmaf(-mean, sl, -r * c_.x));
+        });
+    }
+};
+template <typename T, int VEC, bool GATED, int ACT>
+__device__ __forceinline__ void input_gradient(const Input<T, VEC>& in, const Backward<VEC>& c, Lanes<VEC>& dx, Lanes<VEC>& dg, int rt)
+{
+    const Lanes<VEC> d = Vec<T, VEC>::unpack(in.dy), u = Vec<T, VEC>::unpack(in.x);
+    if constexpr (!GATED)
+    {
+#pragma unroll
+        for (int k = 0; k < Lanes<VEC>::N; ++k)
+        {
+            const float2 dz = act_grad<T, ACT>(fma2(u.p[k], c.scale.p[k], c.shift.p[k]), d.p[k], rt);
+            dx.p[k] = fma2(dz, c.scale.p[k], fma2(u.p[k], c.slope.p[k], c.offset.p[k]));
+        }
+    }
+    else
+    {
+        const Lanes<VEC> g = Vec<T, VEC>::unpack(in.g);
+#pragma unroll
+        for (int k = 0; k < Lanes<VEC>::N; ++k)
+        {
+            float2 value, slope, s, ns;
+            act_both<T, ACT>(u.p[k], value, slope, rt);
+            sigmoid_pair(g.p[k], s, ns);
+            const float2 vs = mul(value, s);
+            const float2 du = fma2(d.p[k], c.scale.p[k], fma2(vs, c.slope.p[k], c.offset.p[k]));
+            dx.p[k] = mul(du, mul(slope, s));
+            dg.p[k] = mul(du, mul(vs, ns));
+        }
+    }
+}
+// channel sums chan[2][C] from the slots' (a row may hold several pixels), then f(g, the group's sums of w dz and w dz uhat)
+template <int VEC, class F>
+__device__ __forceinline__ void channel_and_group_sums(const NormArgs& a, const float* params, const float* buf, float* chan, F f)
+{
+    const int T = blockDim.x, t = threadIdx.x, rows = sum_rows(a);
+    for (int i = t; i < 2 * a.C; i += T)
+    {
+        const int k = i >= a.C, c = i - k * a.C;
+        float s = 0.f;
+        for (int q = 0; q < a.ppr; ++q)
+        {
+            const int e = q * a.C + c;
+            const float* col = buf + (k * VEC + e % VEC) * rows * a.P + e / VEC;
+#pragma unroll 4
+            for (int r = 0; r < rows; ++r) s += col[r * a.P];
+        }
+        chan[i] = s;
+    }
+    __syncthreads();
+    const int lanes = 1 << a.lanes, want = ((a.G << a.lanes) + 31) & ~31;
+    for (int idx = t; idx < want; idx += T)
+    {
+        const int g = idx >> a.lanes, lane = idx & (lanes - 1);
         double s = 0.0, q = 0.0;
         if (g < a.G)
-            for (int i = lane; i < n; i += lanes)
+            for (int i = lane; i < a.Cg; i += lanes)
             {
-                const int e = i / run * a.C + g * a.Cg + i % run * a.m;
-                const int k = (e % VEC) / a.m * a.P + e / VEC;
-                const double piv = (double)pivot[k], ds = (double)tot[k];
-                s += fma(cnt, piv, ds);
-                q += (double)tot[per * a.P + k] + piv * fma(cnt, piv, 2.0 * ds);
+                const int c = g * a.Cg + i;
+                const double w = (double)params[c];
+                s = fma(w, (double)chan[c], s);
+                q = fma(w, (double)chan[a.C + c], q);
             }
         for (int o = lanes >> 1; o > 0; o >>= 1)
         {
             s += __shfl_xor_sync(0xffffffffu, s, o);
             q += __shfl_xor_sync(0xffffffffu, q, o);
         }
-        if (g < a.G && lane == 0) out[g] = make_double2(s, q);
+        if (g < a.G && lane == 0) f(g, make_double2(s, q));
     }
 }
-
-// Sums over the partial sums of an image's groups, by up to eight threads each; scratch of max(G, blockDim) double2. Ends with a barrier.
-__device__ __forceinline__ void gather_groups(const double2* __restrict__ part, int parts, int G, double2* scratch, double2* out)
+// the channels' sums of the cluster's blocks, spread over its threads
+__device__ __forceinline__ void put_channels(cg::cluster_group& cluster, const NormArgs& a, float* chan, float2* out)
 {
-    const int T = blockDim.x, t = threadIdx.x;
-    const int ways = max(1, min(8, min(parts, T / G)));
-    for (int idx = t; idx < ways * G; idx += T)
-    {
-        const int w = idx / G, g = idx % G;
-        double s = 0.0, q = 0.0;
-#pragma unroll 4
-        for (int k = w; k < parts; k += ways)
-        {
-            const double2 v = __ldcg(part + (size_t)k * G + g);
-            s += v.x; q += v.y;
-        }
-        scratch[idx] = make_double2(s, q);
-    }
-    __syncthreads();
-    for (int g = t; g < G; g += T)
-    {
-        double s = 0.0, q = 0.0;
-        for (int w = 0; w < ways; ++w) { s += scratch[w * G + g].x; q += scratch[w * G + g].y; }
-        out[g] = make_double2(s, q);
-    }
-    __syncthreads();
-}
-__device__ __forceinline__ float2 mean_rstd(double2 sums, double n, float eps)
-{
-    const double mean = sums.x / n;
-    double var = sums.y / n - mean * mean;
-    if (var < 0.0) var = 0.0;  // a NaN stays one
-    return make_float2((float)mean, (float)(1.0 / sqrt(var + (double)eps)));
-}
-
-// ---- coefficients of a thread's channels ----------------------------------------------------------------------------------
-template <int VEC> struct Forward
-{
-    float mean[VEC], scale[VEC], shift[VEC];  // z = (u - mean) scale + shift
-    __device__ __forceinline__ void set(const NormArgs& a, int c0, int ph, const float2* stat)
-    {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-        {
-            const int c = (ph * VEC + j) % a.C;
-            const float2 s = stat[c / a.Cg];
-            mean[j] = s.x;
-            scale[j] = a.weight ? s.y * load_param(a.weight, a.param_type, c0 + c) : s.y;
-            shift[j] = a.bias ? load_param(a.bias, a.param_type, c0 + c) : 0.f;
-        }
-    }
-};
-template <typename T, int VEC, bool GATED, int ACT>
-__device__ __forceinline__ void normalise(float (&u)[VEC], const Forward<VEC>& f, int rt)
-{
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-    {
-        const float z = fmaf(u[j] - f.mean[j], f.scale[j], f.shift[j]);
-        u[j] = GATED ? z : act_value<T, ACT>(z, rt);
-    }
-}
-
-// ---- forward, images larger than a cluster's shared memory ------------------------------------------------------------------
-// Shared memory: double2 group[G] | float tot[2 P VEC / m] | pivot[P VEC / m] | block_sums' scratch
-template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const __grid_constant__ NormArgs a)
-{
-    extern __shared__ double2 smem[];
-    let_next_start();
-    const int t = threadIdx.x, T_ = blockDim.x, b = a.image0 + blockIdx.y;
-    int begin, end;
-    chunk_of(a.rows, blockIdx.x, gridDim.x, begin, end);
-    const int slots = a.P * (VEC / a.m);
-    double2* group = smem;
-    float* tot = reinterpret_cast<float*>(group + a.G);
-    float* pivot = tot + 2 * slots;
-    float* buf = pivot + slots;
-    constexpr int U = GATED ? 2 : 4;
-    using V = Vec<T, VEC>;
-    using L = Loaded<T, VEC, GATED>;
-    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
-    {
-        Place pl;
-        pl.ph = a.R == 1 ? ph0 + t : t % a.P;
-        pl.r0 = a.R == 1 ? 0 : t / a.P;
-        pl.active = pl.ph < a.P && pl.r0 < a.R;
-        float v[2][VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[0][j] = v[1][j] = 0.f;
-        if (pl.active)
-        {
-            const T* px = at<T>(a.x, b, 0, begin, pl.ph, VEC);
-            const T* pg = GATED ? at<T>(a.gate, b, 0, begin, pl.ph, VEC) : nullptr;
-            float piv[VEC];
-            {
-                L in;
-                in.x = V::load(px);
-                if (GATED) in.g = V::load(pg);
-                value_of<T, VEC, GATED, ACT>(in, piv, a.act);
-                // one pivot for the channels that are added up together
-#pragma unroll
-                for (int j = 1; j < VEC; ++j)
-                    if (j & (a.m - 1)) piv[j] = piv[j - 1];
-                if (pl.r0 == 0)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if ((j & (a.m - 1)) == 0) pivot[j / a.m * a.P + pl.ph] = piv[j];
-            }
-            for (int r = begin + pl.r0; r < end; r += U * a.R)
-            {
-                L in[U];
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (r + k * a.R < end)
-                    {
-                        const int64_t off = (int64_t)(r + k * a.R - begin);
-                        in[k].x = V::load(px + off * a.x.row);
-                        if (GATED) in[k].g = V::load(pg + off * a.gate.row);
-                    }
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (r + k * a.R < end)
-                    {
-                        float u[VEC];
-                        value_of<T, VEC, GATED, ACT>(in[k], u, a.act);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j)
-                        {
-                            const float d = u[j] - piv[j];
-                            v[0][j] += d;
-                            v[1][j] = fmaf(d, d, v[1][j]);
-                        }
-                    }
-            }
-        }
-        block_sums<VEC>(v, a.m, a, pl, tot, buf);
-    }
-    __syncthreads();
-    group_sums<VEC>(a, end - begin, tot, pivot, group);
-    auto cluster = cg::this_cluster();
-    cluster.sync();
     const int k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    double2* out = a.group_part + ((size_t)b * a.clusters + blockIdx.x / k) * a.G;
-    for (int g = rank * T_ + t; g < a.G; g += k * T_)
+    for (int c = rank * blockDim.x + threadIdx.x; c < a.C; c += k * blockDim.x)
     {
-        double s = 0.0, q = 0.0;
+        float s = 0.f, q = 0.f;
         for (int o = 0; o < k; ++o)
         {
-            const double2 p = cluster.map_shared_rank(group, o)[g];
-            s += p.x; q += p.y;
+            const float* p = cluster.map_shared_rank(chan, o);
+            s += p[c]; q += p[a.C + c];
         }
-        out[g] = make_double2(s, q);
-    }
-    cluster.sync();
-    wait_previous();
-}
-
-// Shared memory: double2 total[G] | scratch[max(G, blockDim)] | float2 stat[G]
-template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_apply(const __grid_constant__ NormArgs a)
-{
-    extern __shared__ double2 smem[];
-    let_next_start();
-    const int t = threadIdx.x, T_ = blockDim.x, b = a.image0 + blockIdx.y;
-    int begin, end;
-    chunk_of(a.rows, blockIdx.x, gridDim.x, begin, end);
-    double2* total = smem;
-    float2* stat = reinterpret_cast<float2*>(smem + a.G + max(a.G, T_));
-    wait_previous();
-    gather_groups(a.group_part + (size_t)b * a.clusters * a.G, a.clusters, a.G, smem + a.G, total);
-    const double n = (double)a.rows * a.ppr * a.Cg;
-    for (int g = t; g < a.G; g += T_)
-    {
-        const float2 s = mean_rstd(total[g], n, a.eps);
-        stat[g] = s;
-        if (a.mean && blockIdx.x == 0)
-        {
-            a.mean[(size_t)b * a.G + g] = s.x;
-            a.rstd[(size_t)b * a.G + g] = s.y;
-        }
-    }
-    __syncthreads();
-    constexpr int U = GATED ? 2 : 4;
-    using V = Vec<T, VEC>;
-    using L = Loaded<T, VEC, GATED>;
-    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
-    {
-        const int ph = a.R == 1 ? ph0 + t : t % a.P, r0 = a.R == 1 ? 0 : t / a.P;
-        if (ph >= a.P || r0 >= a.R) continue;
-        Forward<VEC> f;
-        f.set(a, 0, ph, stat);
-        const T* px = at<T>(a.x, b, 0, 0, ph, VEC);
-        const T* pg = GATED ? at<T>(a.gate, b, 0, 0, ph, VEC) : nullptr;
-        T* py = at_out<T>(a.y, b, 0, 0, ph, VEC);
-        // from the end: what the sums read last is what the L2 still has
-        for (int r = end - 1 - r0; r >= begin; r -= U * a.R)
-        {
-            L in[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r - k * a.R >= begin)
-                {
-                    in[k].x = V::load(px + (int64_t)(r - k * a.R) * a.x.row);
-                    if (GATED) in[k].g = V::load(pg + (int64_t)(r - k * a.R) * a.gate.row);
-                }
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r - k * a.R >= begin)
-                {
-                    float u[VEC];
-                    value_of<T, VEC, GATED, ACT>(in[k], u, a.act);
-                    normalise<T, VEC, GATED, ACT>(u, f, a.act);
-                    V::store(py + (int64_t)(r - k * a.R) * a.y.row, u);
-                }
-        }
+        out[c] = make_float2(s, q);
     }
 }
 
-// ---- backward, images larger than a cluster's shared memory -----------------------------------------------------------------
-// uhat and dz of a vector: z = uhat w + b
-template <int VEC> struct Saved
-{
-    float mean[VEC], rstd[VEC], w[VEC], bias[VEC];
-    __device__ __forceinline__ void set(const NormArgs& a, int c0, int ph, const float* mean_, const float* rstd_)
-    {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-        {
-            const int c = (ph * VEC + j) % a.C, g = c / a.Cg;
-            mean[j] = mean_[g];
-            rstd[j] = rstd_[g];
-            w[j] = a.weight ? load_param(a.weight, a.param_type, c0 + c) : 1.f;
-            bias[j] = a.bias ? load_param(a.bias, a.param_type, c0 + c) : 0.f;
-        }
-    }
-};
-template <typename T, int VEC, bool GATED, int ACT>
-__device__ __forceinline__ void add_grad_sums(const Loaded<T, VEC, GATED>& in, const typename Vec<T, VEC>::W& dy, const Saved<VEC>& s, float (&v)[2][VEC], int rt)
-{
-    float u[VEC], d[VEC];
-    value_of<T, VEC, GATED, ACT>(in, u, rt);
-    Vec<T, VEC>::unpack(dy, d);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-    {
-        const float uhat = (u[j] - s.mean[j]) * s.rstd[j];
-        const float dz = GATED ? d[j] : act_grad<T, ACT>(fmaf(uhat, s.w[j], s.bias[j]), d[j], rt);
-        v[0][j] += dz;
-        v[1][j] = fmaf(dz, uhat, v[1][j]);
-    }
-}
-// du = dz scale + (u - mean) slope + offset, with scale = rstd w, slope = -rstd^2 c2, offset = -rstd c1
-template <int VEC> struct Backward
-{
-    float mean[VEC], scale[VEC], bias[VEC], slope[VEC], offset[VEC];
-    __device__ __forceinline__ void set(const NormArgs& a, int c0, int ph, const float* mean_, const float* rstd_, const float2* c12)
-    {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-        {
-            const int c = (ph * VEC + j) % a.C, g = c / a.Cg;
-            const float r = rstd_[g];
-            mean[j] = mean_[g];
-            scale[j] = a.weight ? r * load_param(a.weight, a.param_type, c0 + c) : r;
-            bias[j] = a.bias ? load_param(a.bias, a.param_type, c0 + c) : 0.f;
-            slope[j] = -r * r * c12[g].y;
-            offset[j] = -r * c12[g].x;
-        }
-    }
-};
-template <typename T, int VEC, bool GATED, int ACT>
-__device__ __forceinline__ void input_gradient(const Loaded<T, VEC, GATED>& in, const typename Vec<T, VEC>::W& dy, const Backward<VEC>& k, float (&dx)[VEC],
-                                               float (&dg)[VEC], int rt)
-{
-    float d[VEC], u[VEC];
-    Vec<T, VEC>::unpack(in.x, u);
-    Vec<T, VEC>::unpack(dy, d);
-    if constexpr (!GATED)
-    {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-        {
-            const float x = u[j] - k.mean[j];
-            const float dz = act_grad<T, ACT>(fmaf(x, k.scale[j], k.bias[j]), d[j], rt);
-            dx[j] = fmaf(dz, k.scale[j], fmaf(x, k.slope[j], k.offset[j]));
-        }
-    }
-    else
-    {
-        float g[VEC];
-        Vec<T, VEC>::unpack(in.g, g);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-        {
-            float value, slope, s, ns;
-            act_both<T, ACT>(u[j], value, slope, rt);
-            sigmoid_pair(g[j], s, ns);
-            const float du = fmaf(d[j], k.scale[j], fmaf(value * s - k.mean[j], k.slope[j], k.offset[j]));
-            dx[j] = du * slope * s;
-            dg[j] = du * value * s * ns;
-        }
-    }
-}
-// channel sums [2][C] from the slots' (a row may hold several pixels), then the groups' sums of w dz and w dz uhat
-template <int VEC>
-__device__ __forceinline__ void channel_and_group_sums(const NormArgs& a, int c0, const float* tot, float* chan, double2* group)
-{
-    const int T = blockDim.x, t = threadIdx.x;
-    for (int i = t; i < 2 * a.C; i += T)
-    {
-        const int k = i / a.C, c = i % a.C;
-        float s = 0.f;
-        for (int q = 0; q < a.ppr; ++q)
-        {
-            const int e = q * a.C + c;
-            s += tot[(k * VEC + e % VEC) * a.P + e / VEC];
-        }
-        chan[i] = s;
-    }
-    __syncthreads();
-    const int want = (a.G * a.lanes + 31) & ~31;
-    for (int idx = t; idx < want; idx += T)
-    {
-        const int g = idx / a.lanes, lane = idx & (a.lanes - 1);
-        double s = 0.0, q = 0.0;
-        if (g < a.G)
-            for (int i = lane; i < a.Cg; i += a.lanes)
-            {
-                const int c = g * a.Cg + i;
-                const double w = a.weight ? (double)load_param(a.weight, a.param_type, c0 + c) : 1.0;
-                s = fma(w, (double)chan[c], s);
-                q = fma(w, (double)chan[a.C + c], q);
-            }
-        for (int o = a.lanes >> 1; o > 0; o >>= 1)
-        {
-            s += __shfl_xor_sync(0xffffffffu, s, o);
-            q += __shfl_xor_sync(0xffffffffu, q, o);
-        }
-        if (g < a.G && lane == 0) group[g] = make_double2(s, q);
-    }
-}
-
-// Shared memory: double2 group[G] | float chan[2 C] | tot[2 P VEC] | block_sums' scratch
+// Shared memory: float2 stat[G] | float params[2 C] | chan[2 C] | block_sums' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad_sums(const __grid_constant__ NormArgs a)
 {
     extern __shared__ double2 smem[];
     let_next_start();
-    const int t = threadIdx.x, T_ = blockDim.x, b = a.image0 + blockIdx.y;
+    const int b = a.image0 + blockIdx.y;
     int begin, end;
-    chunk_of(a.rows, blockIdx.x, gridDim.x, begin, end);
-    double2* group = smem;
-    float* chan = reinterpret_cast<float*>(group + a.G);
-    float* tot = chan + 2 * a.C;
-    float* buf = tot + 2 * a.P * VEC;
-    constexpr int U = 2;
-    using V = Vec<T, VEC>;
-    using L = Loaded<T, VEC, GATED>;
-    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
+    chunk_of(a, blockIdx.x, begin, end);
+    float2* stat = reinterpret_cast<float2*>(smem);
+    float* params = reinterpret_cast<float*>(stat + a.G);
+    float* chan = params + 2 * a.C;
+    float* buf = chan + 2 * a.C;
+    for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
-        Place pl;
-        pl.ph = a.R == 1 ? ph0 + t : t % a.P;
-        pl.r0 = a.R == 1 ? 0 : t / a.P;
-        pl.active = pl.ph < a.P && pl.r0 < a.R;
-        float v[2][VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[0][j] = v[1][j] = 0.f;
+        const Place pl(a, ph0);
+        Stream<T, VEC, GATED, true> in(a, b, pl, begin, end, false, smem);
+        in.start();
+        if (ph0 == 0)
+        {
+            stage_params(a, 0, params);
+            stage_stats(a, (size_t)b * a.G, stat);
+            __syncthreads();
+        }
+        Lanes<VEC> v[2];
+        v[0].fill(0.f); v[1].fill(0.f);
         if (pl.active)
         {
             Saved<VEC> s;
-            s.set(a, 0, pl.ph, a.mean + (size_t)b * a.G, a.rstd + (size_t)b * a.G);
-            const T* px = at<T>(a.x, b, 0, 0, pl.ph, VEC);
-            const T* pg = GATED ? at<T>(a.gate, b, 0, 0, pl.ph, VEC) : nullptr;
-            const T* pd = at<T>(a.dy, b, 0, 0, pl.ph, VEC);
-            for (int r = begin + pl.r0; r < end; r += U * a.R)
-            {
-                L in[U];
-                typename V::W dy[U];
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (r + k * a.R < end)
-                    {
-                        const int64_t row = r + k * a.R;
-                        in[k].x = V::load(px + row * a.x.row);
-                        if (GATED) in[k].g = V::load(pg + row * a.gate.row);
-                        dy[k] = V::load(pd + row * a.dy.row);
-                    }
-#pragma unroll
-                for (int k = 0; k < U; ++k)
-                    if (r + k * a.R < end) add_grad_sums<T, VEC, GATED, ACT>(in[k], dy[k], s, v, a.act);
-            }
+            s.set(a, pl.ph, stat, params);
+            in.run([&](const Input<T, VEC>& i) { add_grad_sums<T, VEC, GATED, ACT>(i, s, v, a.act); });
         }
-        block_sums<VEC>(v, 1, a, pl, tot, buf);
+        block_sums<VEC>(v, 1, a, pl, buf);
     }
     __syncthreads();
-    channel_and_group_sums<VEC>(a, 0, tot, chan, group);
-    auto cluster = cg::this_cluster();
-    cluster.sync();
-    const int k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const size_t part = (size_t)b * a.clusters + blockIdx.x / k;
-    for (int g = rank * T_ + t; g < a.G; g += k * T_)
-    {
-        double s = 0.0, q = 0.0;
-        for (int o = 0; o < k; ++o)
-        {
-            const double2 p = cluster.map_shared_rank(group, o)[g];
-            s += p.x; q += p.y;
-        }
-        a.group_part[part * a.G + g] = make_double2(s, q);
-    }
+    const size_t part = (size_t)b * a.chunks + blockIdx.x;
+    float2* out = a.group_part + (size_t)b * a.chunks * a.G + blockIdx.x;
+    channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { out[(size_t)g * a.chunks] = make_float2((float)sums.x, (float)sums.y); });
     if (a.channel_part)
-        for (int c = rank * T_ + t; c < a.C; c += k * T_)
-        {
-            float s = 0.f, q = 0.f;
-            for (int o = 0; o < k; ++o)
-            {
-                const float* p = cluster.map_shared_rank(chan, o);
-                s += p[c]; q += p[a.C + c];
-            }
-            a.channel_part[part * a.C + c] = make_float2(s, q);
-        }
-    cluster.sync();
+        for (int c = threadIdx.x; c < a.C; c += blockDim.x) a.channel_part[part * a.C + c] = make_float2(chan[c], chan[a.C + c]);
     wait_previous();
 }
 
-// db and dw of up to blockDim channels from `parts` partial sums each, in 64 bits and in a fixed order. Scratch: 2 blockDim double.
+// db and dw of nc channels from c0 on, of `channels` in all, from the partial sums of each, in 64 bits and in a fixed order.
+// Scratch: 2 blockDim double.
 __device__ __forceinline__ void param_gradients(const NormArgs& a, int channels, int c0, int nc, double* scratch)
 {
     const int T = blockDim.x, t = threadIdx.x, ways = T / nc;
-    const int c = t % nc, w = t / nc;
+    const int w = t / nc, c = t - w * nc;
     double s = 0.0, q = 0.0;
     if (w < ways)
 #pragma unroll 8
@@ -778,18 +964,17 @@ __device__ __forceinline__ void param_gradients(const NormArgs& a, int channels,
         if (a.dweight) store_param(a.dweight, a.param_type, c0 + t, (float)q);
     }
 }
-constexpr int kParamChannels = 32;  // channels that one block adds up
 
-// Shared memory: as k_norm_apply; the parameter blocks 2 blockDim double
+// Shared memory: float2 c12[G] | stat[G] | float params[2 C] | vectors; the parameter blocks 2 blockDim double
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad_apply(const __grid_constant__ NormArgs a)
 {
     extern __shared__ double2 smem[];
     let_next_start();
-    const int t = threadIdx.x, T_ = blockDim.x, b = a.image0 + blockIdx.y;
-    wait_previous();
+    const int T_ = blockDim.x, b = a.image0 + blockIdx.y;
     if ((int)blockIdx.x < a.param_blocks)
     {
+        wait_previous();
         if (blockIdx.y == 0)
         {
             const int c0 = blockIdx.x * kParamChannels;
@@ -798,144 +983,321 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         return;
     }
     int begin, end;
-    chunk_of(a.rows, blockIdx.x - a.param_blocks, gridDim.x - a.param_blocks, begin, end);
-    float2* c12 = reinterpret_cast<float2*>(smem + a.G + max(a.G, T_));
-    gather_groups(a.group_part + (size_t)b * a.clusters * a.G, a.clusters, a.G, smem + a.G, smem);
-    const double n = (double)a.rows * a.ppr * a.Cg;
-    for (int g = t; g < a.G; g += T_) c12[g] = make_float2((float)(smem[g].x / n), (float)(smem[g].y / n));
-    __syncthreads();
-    constexpr int U = 2;
-    using V = Vec<T, VEC>;
-    using L = Loaded<T, VEC, GATED>;
+    chunk_of(a, blockIdx.x - a.param_blocks, begin, end);
+    float2* c12 = reinterpret_cast<float2*>(smem);
+    float2* stat = c12 + a.G;
+    float* params = reinterpret_cast<float*>(stat + a.G);
     for (int ph0 = 0; ph0 < a.P; ph0 += T_)
     {
-        const int ph = a.R == 1 ? ph0 + t : t % a.P, r0 = a.R == 1 ? 0 : t / a.P;
-        if (ph >= a.P || r0 >= a.R) continue;
-        Backward<VEC> c;
-        c.set(a, 0, ph, a.mean + (size_t)b * a.G, a.rstd + (size_t)b * a.G, c12);
-        const T* px = at<T>(a.x, b, 0, 0, ph, VEC);
-        const T* pg = GATED ? at<T>(a.gate, b, 0, 0, ph, VEC) : nullptr;
-        const T* pd = at<T>(a.dy, b, 0, 0, ph, VEC);
-        T* pdx = at_out<T>(a.dx, b, 0, 0, ph, VEC);
-        T* pdg = GATED ? at_out<T>(a.dgate, b, 0, 0, ph, VEC) : nullptr;
-        for (int r = end - 1 - r0; r >= begin; r -= U * a.R)
+        const Place pl(a, ph0);
+        Stream<T, VEC, GATED, true> in(a, b, pl, begin, end, true, smem);
+        in.start();
+        if (ph0 == 0)
         {
-            L in[U];
-            typename V::W dy[U];
+            stage_params(a, 0, params);
+            stage_stats(a, (size_t)b * a.G, stat);
+            wait_previous();
+            gather_groups(
+                a, b, [&](int, float2 v) { return make_double2(v.x, v.y); },
+                [&](int g, double2 sums) { c12[g] = make_float2((float)(sums.x * a.inv_n), (float)(sums.y * a.inv_n)); });
+            __syncthreads();
+        }
+        if (!pl.active) continue;
+        Backward<VEC> c;
+        c.set(a, pl.ph, stat, c12, params);
+        Walk<T> dx(a.dx, b, 0, pl, a.R, VEC, begin, end, true), dg(a.dgate, b, 0, pl, a.R, VEC, begin, end, true);
+        in.run([&](const Input<T, VEC>& i) {
+            Lanes<VEC> o, og;
+            input_gradient<T, VEC, GATED, ACT>(i, c, o, og, a.act);
+            Vec<T, VEC>::store(dx.p, o);
+            dx.on(1);
+            if constexpr (GATED)
+            {
+                Vec<T, VEC>::store(dg.p, og);
+                dg.on(1);
+            }
+        });
+    }
+}
+
+// ---- images that fit a cluster's shared memory ------------------------------------------------------------------------------
+// A cluster of blocks keeps one image, or some groups' channels of it, in shared memory between the sums and what follows: every
+// value is read from global memory once. A thread copies, reads and overwrites vectors of its own only.
+// n vectors in four groups: all copies are under way before the first group is used
+template <class Copy, class Between, class Use> __device__ __forceinline__ void staged(int n, int most, Copy copy, Between between, Use use)
+{
+    const int quarter = (most + 3) / 4;
 #pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r - k * a.R >= begin)
+    for (int q = 0; q < 4; ++q)
+    {
+        for (int i = q * quarter; i < min(n, (q + 1) * quarter); ++i) copy(i);
+        copies_commit();
+    }
+    between();
+    copies_wait<3>();
+    for (int i = 0; i < min(n, quarter); ++i) use(i);
+    copies_wait<2>();
+    for (int i = quarter; i < min(n, 2 * quarter); ++i) use(i);
+    copies_wait<1>();
+    for (int i = 2 * quarter; i < min(n, 3 * quarter); ++i) use(i);
+    copies_wait<0>();
+    for (int i = 3 * quarter; i < n; ++i) use(i);
+}
+
+// Shared memory: double2 group[G] | float2 stat[G] | float params[2 C] | pivots[P VEC / m] | block_sums' scratch | vectors
+template <typename T, int VEC, bool GATED, int ACT>
+__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(const __grid_constant__ NormArgs a)
+{
+    extern __shared__ double2 smem[];
+    auto cluster = cg::this_cluster();
+    const int t = threadIdx.x, T_ = blockDim.x, k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = blockIdx.y >> a.slices, slice = blockIdx.y - (b << a.slices), c0 = slice * a.C;
+    int begin, end;
+    chunk_of(a, rank, begin, end);
+    double2* group = smem;
+    float2* stat = reinterpret_cast<float2*>(group + a.G);
+    float* params = reinterpret_cast<float*>(stat + a.G);
+    float* shared = params + 2 * a.C;
+    float* buf = shared + a.P * (VEC / a.m);
+    using V = Vec<T, VEC>;
+    using W = typename V::W;
+    using In = Input<T, VEC>;
+    const int most = (end - begin + a.R - 1) / a.R;
+    W* sx = reinterpret_cast<W*>(reinterpret_cast<char*>(smem) + a.vectors) + t;
+    W* sg = sx + (size_t)most * T_;
+    const Place pl(a, 0);
+    const int n = pl.active ? pl.count(a, begin, end) : 0;
+    constexpr int H = Lanes<VEC>::N / 2;  // u in 32 bits takes the room of x and of the gate, or of x alone
+    Lanes<VEC> v[2], pivot;
+    v[0].fill(0.f); v[1].fill(0.f); pivot.fill(0.f);
+    const Walk<T> x(a.x, b, c0, pl, a.R, VEC, begin, end, false), g(a.gate, b, c0, pl, a.R, VEC, begin, end, false);
+    bool have = false;
+    staged(
+        n, most,
+        [&](int i) {
+            copy_async<V::kBytes>(sx + i * T_, x.at(i));
+            if constexpr (GATED) copy_async<V::kBytes>(sg + i * T_, g.at(i));
+        },
+        [&] { stage_params(a, c0, params); },
+        [&](int i) {
+            In in;
+            in.x = sx[i * T_];
+            if constexpr (GATED) in.g = sg[i * T_];
+            const Lanes<VEC> u = value_of<T, VEC, GATED, ACT>(in, a.act);
+            if (!have) pivot = pivot_of<VEC>(u, a.m);
+            have = true;
+            add_moments<VEC>(u, pivot, v);
+            if constexpr (GATED)
+            {
+                if constexpr (sizeof(T) == 4) sx[i * T_] = *reinterpret_cast<const W*>(&u);
+                else
                 {
-                    const int64_t row = r - k * a.R;
-                    in[k].x = V::load(px + row * a.x.row);
-                    if (GATED) in[k].g = V::load(pg + row * a.gate.row);
-                    dy[k] = V::load(pd + row * a.dy.row);
+                    sx[i * T_] = *reinterpret_cast<const W*>(&u.p[0]);
+                    sg[i * T_] = *reinterpret_cast<const W*>(&u.p[H]);
                 }
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r - k * a.R >= begin)
-                {
-                    const int64_t row = r - k * a.R;
-                    float dx[VEC], dg[VEC];
-                    input_gradient<T, VEC, GATED, ACT>(in[k], dy[k], c, dx, dg, a.act);
-                    V::store(pdx + row * a.dx.row, dx);
-                    if (GATED) V::store(pdg + row * a.dgate.row, dg);
-                }
+            }
+        });
+    common_pivot<VEC>(v, pivot, n, a, pl, shared);
+    block_sums<VEC>(v, a.m, a, pl, buf);
+    __syncthreads();
+    group_sums<VEC>(a, end - begin, buf, shared, [&](int g, double2 sums) { group[g] = sums; });
+    if (k > 1) cluster.sync();
+    else __syncthreads();
+    const size_t g0 = (((size_t)b << a.slices) + slice) * a.G;
+    for (int i = t; i < a.G; i += T_)
+    {
+        const float2 s = mean_rstd(cluster_sum(cluster, group, i), a.inv_n, a.eps);
+        stat[i] = s;
+        if (a.mean && rank == 0)
+        {
+            a.mean[g0 + i] = s.x;
+            a.rstd[g0 + i] = s.y;
         }
     }
+    __syncthreads();
+    if (k > 1) cluster.barrier_arrive();
+    if (n > 0)
+    {
+        Forward<VEC> f;
+        f.set(a, pl.ph, stat, params);
+        const Walk<T> y(a.y, b, c0, pl, a.R, VEC, begin, end, false);
+#pragma unroll 2
+        for (int i = 0; i < n; ++i)
+        {
+            Lanes<VEC> u;
+            const W w = sx[i * T_];
+            if constexpr (!GATED) u = V::unpack(w);
+            else if constexpr (sizeof(T) == 4) *reinterpret_cast<W*>(&u) = w;
+            else
+            {
+                *reinterpret_cast<W*>(&u.p[0]) = w;
+                *reinterpret_cast<W*>(&u.p[H]) = sg[i * T_];
+            }
+            normalise<T, VEC, GATED, ACT>(u, f, a.act);
+            V::store(y.at(i), u);
+        }
+    }
+    if (k > 1) cluster.barrier_wait();  // nobody leaves while its sums may still be read
+}
+
+// Shared memory: double2 group[G] | float2 c12[G] | stat[G] | float params[2 C] | chan[2 C] | block_sums' scratch | vectors
+template <typename T, int VEC, bool GATED, int ACT>
+__global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad_resident(const __grid_constant__ NormArgs a)
+{
+    extern __shared__ double2 smem[];
+    let_next_start();
+    auto cluster = cg::this_cluster();
+    const int t = threadIdx.x, T_ = blockDim.x, k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int b = blockIdx.y >> a.slices, slice = blockIdx.y - (b << a.slices), c0 = slice * a.C;
+    int begin, end;
+    chunk_of(a, rank, begin, end);
+    double2* group = smem;
+    float2* c12 = reinterpret_cast<float2*>(group + a.G);
+    float2* stat = c12 + a.G;
+    float* params = reinterpret_cast<float*>(stat + a.G);
+    float* chan = params + 2 * a.C;
+    float* buf = chan + 2 * a.C;
+    using V = Vec<T, VEC>;
+    using W = typename V::W;
+    using In = Input<T, VEC>;
+    const int most = (end - begin + a.R - 1) / a.R;
+    W* sx = reinterpret_cast<W*>(reinterpret_cast<char*>(smem) + a.vectors) + t;
+    W* sd = sx + (size_t)most * T_;
+    W* sg = sd + (size_t)most * T_;
+    const Place pl(a, 0);
+    const int n = pl.active ? pl.count(a, begin, end) : 0;
+    auto get = [&](int i) {
+        In in;
+        in.x = sx[i * T_];
+        in.dy = sd[i * T_];
+        if constexpr (GATED) in.g = sg[i * T_];
+        return in;
+    };
+    Lanes<VEC> v[2];
+    v[0].fill(0.f); v[1].fill(0.f);
+    {
+        const Walk<T> x(a.x, b, c0, pl, a.R, VEC, begin, end, false), g(a.gate, b, c0, pl, a.R, VEC, begin, end, false),
+            d(a.dy, b, c0, pl, a.R, VEC, begin, end, false);
+        Saved<VEC> s;
+        staged(
+            n, most,
+            [&](int i) {
+                copy_async<V::kBytes>(sx + i * T_, x.at(i));
+                copy_async<V::kBytes>(sd + i * T_, d.at(i));
+                if constexpr (GATED) copy_async<V::kBytes>(sg + i * T_, g.at(i));
+            },
+            [&] {
+                stage_params(a, c0, params);
+                stage_stats(a, (((size_t)b << a.slices) + slice) * a.G, stat);
+                __syncthreads();
+                if (pl.active) s.set(a, pl.ph, stat, params);
+            },
+            [&](int i) { add_grad_sums<T, VEC, GATED, ACT>(get(i), s, v, a.act); });
+    }
+    block_sums<VEC>(v, 1, a, pl, buf);
+    __syncthreads();
+    channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { group[g] = sums; });
+    if (k > 1) cluster.sync();
+    else __syncthreads();
+    for (int i = t; i < a.G; i += T_)
+    {
+        const double2 s = cluster_sum(cluster, group, i);
+        c12[i] = make_float2((float)(s.x * a.inv_n), (float)(s.y * a.inv_n));
+    }
+    if (a.channel_part) put_channels(cluster, a, chan, a.channel_part + (((size_t)b << a.slices) + slice) * a.C);
+    __syncthreads();
+    if (k > 1) cluster.barrier_arrive();
+    if (n > 0)
+    {
+        Backward<VEC> c;
+        c.set(a, pl.ph, stat, c12, params);
+        const Walk<T> dx(a.dx, b, c0, pl, a.R, VEC, begin, end, false), dg(a.dgate, b, c0, pl, a.R, VEC, begin, end, false);
+        for (int i = 0; i < n; ++i)
+        {
+            Lanes<VEC> o, og;
+            input_gradient<T, VEC, GATED, ACT>(get(i), c, o, og, a.act);
+            V::store(dx.at(i), o);
+            if constexpr (GATED) V::store(dg.at(i), og);
+        }
+    }
+    if (k > 1) cluster.barrier_wait();
+}
+// the parameters' gradients behind it: [B, slices * C] partial sums. Shared memory: 2 blockDim double
+template <typename T> __global__ void __launch_bounds__(kNormGradThreads) k_norm_grad_params(const __grid_constant__ NormArgs a)
+{
+    extern __shared__ double2 smem[];
+    wait_previous();
+    const int channels = a.C << a.slices, c0 = blockIdx.x * kParamChannels;
+    param_gradients(a, channels, c0, min(kParamChannels, channels - c0), reinterpret_cast<double*>(smem));
 }
 
 // ---- the gate alone -----------------------------------------------------------------------------------------------------
 template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_gate(const __grid_constant__ NormArgs a)
+__global__ void __launch_bounds__(kGateThreads, kGateBlocks) k_gate(const __grid_constant__ NormArgs a)
 {
-    const int t = threadIdx.x, T_ = blockDim.x, b = blockIdx.y;
+    const int b = blockIdx.y;
     int begin, end;
-    chunk_of(a.rows, blockIdx.x, gridDim.x, begin, end);
+    chunk_of(a, blockIdx.x, begin, end);
     constexpr int U = 2;
     using V = Vec<T, VEC>;
-    using L = Loaded<T, VEC, true>;
-    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
+    using In = Input<T, VEC>;
+    for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
-        const int ph = a.R == 1 ? ph0 + t : t % a.P, r0 = a.R == 1 ? 0 : t / a.P;
-        if (ph >= a.P || r0 >= a.R) continue;
-        const T* px = at<T>(a.x, b, 0, 0, ph, VEC);
-        const T* pg = at<T>(a.gate, b, 0, 0, ph, VEC);
-        T* py = at_out<T>(a.y, b, 0, 0, ph, VEC);
-        for (int r = begin + r0; r < end; r += U * a.R)
-        {
-            L in[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r + k * a.R < end)
-                {
-                    const int64_t row = r + k * a.R;
-                    in[k].x = V::load(px + row * a.x.row);
-                    in[k].g = V::load(pg + row * a.gate.row);
-                }
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r + k * a.R < end)
-                {
-                    float u[VEC];
-                    value_of<T, VEC, true, ACT>(in[k], u, a.act);
-                    V::store(py + (int64_t)(r + k * a.R) * a.y.row, u);
-                }
-        }
+        const Place pl(a, ph0);
+        if (!pl.active) continue;
+        Walk<T> x(a.x, b, 0, pl, a.R, VEC, begin, end, false), g(a.gate, b, 0, pl, a.R, VEC, begin, end, false), y(a.y, b, 0, pl, a.R, VEC, begin, end, false);
+        batches<U>(
+            pl.count(a, begin, end),
+            [&](int k) {
+                In i;
+                i.x = V::load(x.at(k));
+                i.g = V::load(g.at(k));
+                return i;
+            },
+            [&](int k, const In& i) { V::store(y.at(k), value_of<T, VEC, true, ACT>(i, a.act)); },
+            [&](int k) { x.on(k); g.on(k); y.on(k); });
     }
 }
 template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_gate_grad(const __grid_constant__ NormArgs a)
+__global__ void __launch_bounds__(kGateGradThreads, kGateBlocks) k_gate_grad(const __grid_constant__ NormArgs a)
 {
-    const int t = threadIdx.x, T_ = blockDim.x, b = blockIdx.y;
+    const int b = blockIdx.y;
     int begin, end;
-    chunk_of(a.rows, blockIdx.x, gridDim.x, begin, end);
+    chunk_of(a, blockIdx.x, begin, end);
     constexpr int U = 2;
     using V = Vec<T, VEC>;
-    for (int ph0 = 0; ph0 < a.P; ph0 += T_)
+    using In = Input<T, VEC>;
+    for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
-        const int ph = a.R == 1 ? ph0 + t : t % a.P, r0 = a.R == 1 ? 0 : t / a.P;
-        if (ph >= a.P || r0 >= a.R) continue;
-        const T* px = at<T>(a.x, b, 0, 0, ph, VEC);
-        const T* pg = at<T>(a.gate, b, 0, 0, ph, VEC);
-        const T* pd = at<T>(a.dy, b, 0, 0, ph, VEC);
-        T* pdx = at_out<T>(a.dx, b, 0, 0, ph, VEC);
-        T* pdg = at_out<T>(a.dgate, b, 0, 0, ph, VEC);
-        for (int r = begin + r0; r < end; r += U * a.R)
-        {
-            typename V::W in[U][3];
+        const Place pl(a, ph0);
+        if (!pl.active) continue;
+        Walk<T> x(a.x, b, 0, pl, a.R, VEC, begin, end, false), g(a.gate, b, 0, pl, a.R, VEC, begin, end, false), d(a.dy, b, 0, pl, a.R, VEC, begin, end, false),
+            dx(a.dx, b, 0, pl, a.R, VEC, begin, end, false), dg(a.dgate, b, 0, pl, a.R, VEC, begin, end, false);
+        batches<U>(
+            pl.count(a, begin, end),
+            [&](int k) {
+                In i;
+                i.x = V::load(x.at(k));
+                i.g = V::load(g.at(k));
+                i.dy = V::load(d.at(k));
+                return i;
+            },
+            [&](int k, const In& i) {
+                Lanes<VEC> f = V::unpack(i.x), e = V::unpack(i.g), dy = V::unpack(i.dy);
 #pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r + k * a.R < end)
+                for (int q = 0; q < Lanes<VEC>::N; ++q)
                 {
-                    const int64_t row = r + k * a.R;
-                    in[k][0] = V::load(px + row * a.x.row);
-                    in[k][1] = V::load(pg + row * a.gate.row);
-                    in[k][2] = V::load(pd + row * a.dy.row);
+                    float2 value, slope, s, ns;
+                    act_both<T, ACT>(f.p[q], value, slope, a.act);
+                    sigmoid_pair(e.p[q], s, ns);
+                    const float2 ds = mul(dy.p[q], s);
+                    f.p[q] = mul(ds, slope);
+                    e.p[q] = mul(ds, mul(value, ns));
                 }
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (r + k * a.R < end)
-                {
-                    const int64_t row = r + k * a.R;
-                    float f[VEC], g[VEC], d[VEC];
-                    V::unpack(in[k][0], f);
-                    V::unpack(in[k][1], g);
-                    V::unpack(in[k][2], d);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                    {
-                        float value, slope, s, ns;
-                        act_both<T, ACT>(f[j], value, slope, a.act);
-                        sigmoid_pair(g[j], s, ns);
-                        const float ds = d[j] * s;
-                        f[j] = ds * slope;
-                        g[j] = ds * value * ns;
-                    }
-                    V::store(pdx + row * a.dx.row, f);
-                    V::store(pdg + row * a.dgate.row, g);
-                }
-        }
+                V::store(dx.at(k), f);
+                V::store(dg.at(k), e);
+            },
+            [&](int k) { x.on(k); g.on(k); d.on(k); dx.on(k); dg.on(k); });
     }
 }
 
@@ -948,14 +1310,20 @@ template <typename T, int VEC, bool GATED, int ACT> const void* pick(int which)
         case kNormApply: return (const void*)k_norm_apply<T, VEC, GATED, ACT>;
         case kNormGradSums: return (const void*)k_norm_grad_sums<T, VEC, GATED, ACT>;
         case kNormGradApply: return (const void*)k_norm_grad_apply<T, VEC, GATED, ACT>;
+        case kNormGradParams: return (const void*)k_norm_grad_params<T>;
         case kGate: return (const void*)k_gate<T, VEC, true, ACT>;
         case kGateGrad: return (const void*)k_gate_grad<T, VEC, true, ACT>;
+    }
+    if constexpr (VEC > 1)
+    {
+        if (which == kNormResident) return (const void*)k_norm_resident<T, VEC, GATED, ACT>;
+        if (which == kNormGradResident) return (const void*)k_norm_grad_resident<T, VEC, GATED, ACT>;
     }
     return nullptr;
 }
 template <typename T, int VEC, bool GATED> const void* pick_act(int which, int act)
 {
-    if constexpr (VEC * sizeof(T) == 16)
+    if constexpr (VEC > 1)
         switch (act)
         {
             case ADOP_ACTIVATION_NONE: return pick<T, VEC, GATED, ADOP_ACTIVATION_NONE>(which);

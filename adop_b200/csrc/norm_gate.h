@@ -34,30 +34,38 @@ struct NormImage
 struct NormArgs
 {
     int C, G, Cg;     // channels and groups of a slice; channels of a group
-    int slices;       // independent channel ranges of an image (1 but in the resident kernels)
+    int slices;       // log2 of the independent channel ranges of an image (0 but in the resident kernels)
     int P, ppr;       // vectors and pixels of a row
     int R;            // rows that a block takes at once (1 when a row has more vectors than the block threads)
     int m;            // channels of a thread's vector that share a group: gcd(Cg, VEC)
-    int lanes;        // threads that add up one group's slots (a power of two up to 32)
+    int lanes, row_lanes;  // log2 of the threads that add up one group's sums, and of those for one slot's rows
     int rows;         // rows of an image
     int image0;       // first image of the launch
-    int clusters;     // partial sums of an image
+    int chunks;       // parts of an image, which have a partial sum each
+    int chunk_rows, chunk_more;            // rows of a part; the first chunk_more parts have one more
+    double inv_n, inv_short, inv_long;     // 1 / values of a group in the image, in a part, in one with a row more
+    int gather;           // log2 of the threads that add up a group's partial sums
+    float inv_P, inv_Cg;
     int param_blocks; // blocks of kNormGradApply that add up the parameters' gradients
     int param_parts;  // partial sums of a channel, over all images
+    int vectors;      // bytes of shared memory in front of the vectors
     int act, param_type;
     float eps;
     NormImage x, gate, y, dy, dx, dgate;
     const void *weight, *bias;
     void *dweight, *dbias;
-    float *mean, *rstd;   // [B, slices * G]
-    double2* group_part;  // [B, clusters, G]
-    float2* channel_part; // [B, clusters, C] (resident: [B, 1, slices * C])
+    float *mean, *rstd;   // [B, G of all slices]
+    float2* group_part;   // [B, G, chunks]
+    float2* channel_part; // [B, chunks, C] (resident: [B, 1, C of all slices])
 };
 
 // threads of a block and resident blocks of an SM that the kernels are compiled for
 constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
-constexpr int kNormGradThreads = 256, kNormGradBlocks = 2;  // backward
-constexpr int kNormMaxThreads = 512;
+constexpr int kNormGradThreads = 384, kNormGradBlocks = 2;  // backward
+constexpr int kGateThreads = 512, kGateGradThreads = 256, kGateBlocks = 2;  // the gate alone
+// vectors that the streaming kernels have under way for each thread: a power of two
+__host__ __device__ constexpr int stream_depth(bool gated, bool grad) { return gated ? 4 : 8; }
+constexpr int kParamChannels = 32;  // channels whose parameters' gradients one block adds up
 
 const void* norm_kernel_f32(int which, int vec, bool gated, int act);
 const void* norm_kernel_f16(int which, int vec, bool gated, int act);

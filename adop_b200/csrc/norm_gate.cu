@@ -98,8 +98,10 @@ void threads_of(int P, int most, int* R, int* threads)
     *threads = P > most ? most : (*R * P + 31) / 32 * 32;
 }
 
-// Images whose inputs are read twice, by the sums and by what follows, are taken in groups that the L2 holds.
-constexpr int64_t kL2Group = 64ll << 20;
+// Images whose inputs are read twice, by the sums and by what follows, are taken in groups of which the L2 keeps a good part. A group
+// costs two launches (5 us of waits and tails), so two images go together up to the larger bound. Measured: four images of 33 MB of
+// inputs, backward, two by two 78 us, all at once 82 us; sixteen of 50 MB one by one 418 us, two by two 378 us.
+constexpr int64_t kL2Group = 70ll << 20, kL2Pair = 105ll << 20, kGroupCost = 20ll << 20;
 constexpr int64_t kMinChunk = 16 << 10;  // bytes of one tensor that a block is worth
 
 // How the streaming kernels share out a batch: images of a launch and blocks of an image. By the sizes alone, so that the
@@ -112,11 +114,17 @@ Share share_of(const adop_norm_params* p, bool gated, bool backward)
 {
     const int64_t tensor = p->pixels * p->channels * element_size(p->type);
     const int64_t read = tensor * (1 + (gated ? 1 : 0) + (backward ? 1 : 0));
-    int64_t images = kL2Group / (read > 0 ? read : 1);
-    if (images < 1) images = 1;
-    if (images > p->batch) images = p->batch;
-    const int64_t launches = (p->batch + images - 1) / images;
-    images = (p->batch + launches - 1) / launches;
+    int64_t most = kL2Group / read;
+    if (most < 2 && 2 * read <= kL2Pair) most = 2;
+    if (most > p->batch) most = p->batch;
+    if (most < 1) most = 1;
+    // groups of one size, the last one too: its blocks have as much to do as the others'
+    int64_t images = most, least = -1;
+    for (int64_t n = most; n >= 1 && 2 * n >= most; --n)
+    {
+        const int64_t cost = (p->batch + n - 1) / n * (kGroupCost + n * read);
+        if (least < 0 || cost < least) { least = cost; images = n; }
+    }
     const int64_t wave = (int64_t)sm_count();
     int64_t chunks = wave / images, worth = (tensor + kMinChunk - 1) / kMinChunk;
     if (chunks > worth) chunks = worth;
@@ -205,7 +213,7 @@ adop_status launch(const Launch& l, const adop_norm_params* p, const Shape& sh, 
         int device = 0;
         ADOP_CUDA_TRY(cudaGetDevice(&device));
         ADOP_CUDA_TRY(once[p->type][l.which][sh.vec][gated][p->activation].run(
-            device, [&] { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024); }));
+            device, [&] { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024); }));
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = l.grid;
@@ -213,13 +221,20 @@ adop_status launch(const Launch& l, const adop_norm_params* p, const Shape& sh, 
     cfg.dynamicSmemBytes = l.smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)l.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = l.early ? 2 : 1;
+    if (l.cluster > 1)
+    {
+        cudaLaunchAttribute& c = attr[cfg.numAttrs++];
+        c.id = cudaLaunchAttributeClusterDimension;
+        c.val.clusterDim.x = (unsigned)l.cluster;
+        c.val.clusterDim.y = c.val.clusterDim.z = 1;
+    }
+    if (l.early)
+    {
+        cudaLaunchAttribute& c = attr[cfg.numAttrs++];
+        c.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        c.val.programmaticStreamSerializationAllowed = 1;
+    }
     void* args[] = {&a};
     cudaError_t e = cudaSuccess;
     ADOP_LAUNCH(l.name, st, (e = cudaLaunchKernelExC(&cfg, f, args)));
@@ -326,7 +341,6 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     ADOP_TRY(check_image(p, io->x, false, "x"));
     if (gated) ADOP_TRY(check_image(p, io->gate, false, "gate"));
     ADOP_TRY(check_image(p, io->y, true, "y"));
-    ADOP_TRY(check_workspace(p, io, gated, false));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const adop_norm_image* images[3] = {&io->x, &io->y, &io->gate};
     const Shape sh = choose_shape(p, images, gated ? 3 : 2);
@@ -342,6 +356,7 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
         NormArgs s = slice_args(a, r);
         return launch({"k_norm_resident", kNormResident, r.threads, r.k, dim3((unsigned)r.k, (unsigned)p->batch << r.slices), r.smem, false}, p, sh, gated, s, st);
     }
+    ADOP_TRY(check_workspace(p, io, gated, false));
     int threads;
     threads_of(a.P, kNormThreads, &a.R, &threads);
     const Share share = share_of(p, gated, false);
@@ -386,7 +401,6 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         ADOP_TRY(check_image(p, io->gate, false, "gate"));
         ADOP_TRY(check_image(p, io->grad_gate, true, "grad_gate"));
     }
-    ADOP_TRY(check_workspace(p, io, gated, true));
     const adop_norm_image* images[5] = {&io->x, &io->grad_y, &io->grad_x, &io->gate, &io->grad_gate};
     const Shape sh = choose_shape(p, images, gated ? 5 : 3);
     NormArgs a = args_of(p, sh, true);
@@ -401,6 +415,7 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
     Resident r;
     if (resident_of(p, sh, gated, true, &r))
     {
+        if (params) ADOP_TRY(check_workspace(p, io, gated, true));
         NormArgs s = slice_args(a, r);
         s.channel_part = params ? static_cast<float2*>(io->workspace) : nullptr;
         s.param_parts = p->batch;
@@ -410,6 +425,7 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         return launch({"k_norm_grad_params", kNormGradParams, kNormGradThreads, 1, dim3((unsigned)((a.C + kParamChannels - 1) / kParamChannels)),
                        sizeof(double) * 2 * kNormGradThreads, true}, p, sh, gated, s, st);
     }
+    ADOP_TRY(check_workspace(p, io, gated, true));
     int threads;
     threads_of(a.P, kNormGradThreads, &a.R, &threads);
     const Share share = share_of(p, gated, true);

@@ -159,13 +159,19 @@ __device__ __forceinline__ float rcp(float v)
 __device__ __forceinline__ float2 exp2v(float2 v) { return make_float2(ex2(v.x), ex2(v.y)); }
 __device__ __forceinline__ float2 rcp2(float2 v) { return make_float2(rcp(v.x), rcp(v.y)); }
 __device__ __forceinline__ float2 sigmoid(float2 v) { return rcp2(add(exp2v(mul(v, pair(-kLog2e))), pair(1.f))); }
-// sigmoid s and 1 - s, both to a few units of the last place: from e = exp(-|v|), which never overflows
+// sigmoid s and 1 - s = exp(-v) s, both to a few units of the last place. The exponential stays finite; where it would not, s is 0.
+__device__ __forceinline__ float min_or_nan(float v, float most)
+{
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+    return r;
+}
 __device__ __forceinline__ void sigmoid_pair(float2 v, float2& s, float2& ns)
 {
-    const float2 e = exp2v(mul(make_float2(fabsf(v.x), fabsf(v.y)), pair(-kLog2e)));
-    const float2 t = rcp2(add(e, pair(1.f))), et = mul(e, t);
-    s = make_float2(v.x >= 0.f ? t.x : et.x, v.y >= 0.f ? t.y : et.y);
-    ns = make_float2(v.x >= 0.f ? et.x : t.x, v.y >= 0.f ? et.y : t.y);
+    const float2 m = mul(v, pair(-kLog2e));
+    const float2 e = make_float2(ex2(min_or_nan(m.x, 127.f)), ex2(min_or_nan(m.y, 127.f)));
+    s = rcp2(add(e, pair(1.f)));
+    ns = mul(e, s);
 }
 // v > 0 ? v : exp(v) - 1, with e = exp(v). Near zero, where e - 1 loses digits, the Taylor series: for 16-bit images four terms above
 // -1/16 (the fifth is below 2^-22 of the sum there), for 32 bits eight above -1/2 (the ninth is below 2^-26).
@@ -327,11 +333,14 @@ template <int VEC, class F> __device__ __forceinline__ void for_channels(const N
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from)
+// L1: through the first-level cache. Features and gates that lie side by side share sectors, and where a pixel has few of them the
+// second copy finds its half there (sums over 8 channels of 16 bits 48 -> 36 us for 134 MB); everything else goes past it, as two
+// tensors eight vectors deep do not fit beside the slots (backward sums 114 -> 129 us for 537 MB with it).
+template <int BYTES, bool L1> __device__ __forceinline__ void copy_async(void* to, const void* from)
 {
     const unsigned s = (unsigned)__cvta_generic_to_shared(to);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(s), "l"(from) : "memory");
+    if constexpr (BYTES == 16 && !L1) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(s), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
@@ -360,48 +369,56 @@ template <typename T, int VEC, bool GATED, bool GRAD> struct Stream
           slots(reinterpret_cast<W*>(static_cast<char*>(shared) + a.vectors) + threadIdx.x)
     {
     }
-    __device__ __forceinline__ W* slot(int i) const { return slots + (i & (D - 1)) * kTensors * blockDim.x; }
-    __device__ __forceinline__ void copy(int i)
+    // vectors i, i + 1 of an even i: one group of copies
+    __device__ __forceinline__ W* slot(int i) const { return slots + (i & (D - 1)) * kTensors * (int)blockDim.x; }
+    __device__ __forceinline__ void copy(int i, W* s)
     {
-        W* s = slot(i);
-        copy_async<V::kBytes>(s, x.p);
-        x.on(1);
-        if constexpr (GATED)
-        {
-            copy_async<V::kBytes>(s + blockDim.x, g.p);
-            g.on(1);
-        }
-        if constexpr (GRAD)
-        {
-            copy_async<V::kBytes>(s + (kTensors - 1) * blockDim.x, d.p);
-            d.on(1);
-        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (i + k < n)
+            {
+                W* to = s + k * kTensors * (int)blockDim.x;
+                copy_async<V::kBytes, GATED>(to, x.at(k));
+                if constexpr (GATED) copy_async<V::kBytes, true>(to + blockDim.x, g.at(k));
+                if constexpr (GRAD) copy_async<V::kBytes, false>(to + (kTensors - 1) * (int)blockDim.x, d.at(k));
+            }
+        x.on(2);
+        if constexpr (GATED) g.on(2);
+        if constexpr (GRAD) d.on(2);
+        copies_commit();
+    }
+    __device__ __forceinline__ In get(const W* s) const
+    {
+        In in;
+        in.x = s[0];
+        if constexpr (GATED) in.g = s[blockDim.x];
+        if constexpr (GRAD) in.dy = s[(kTensors - 1) * (int)blockDim.x];
+        return in;
     }
     __device__ __forceinline__ void start()
     {
         if constexpr (VEC > 1)
 #pragma unroll
-            for (int i = 0; i < D; ++i)
-            {
-                if (i < n) copy(i);
-                copies_commit();
-            }
+            for (int i = 0; i < D; i += 2) copy(i, slot(i));
     }
     template <class Use> __device__ __forceinline__ void run(Use use)
     {
         if constexpr (VEC > 1)
         {
-            for (int i = 0; i < n; ++i)
+            int i = 0;
+            for (; i + 1 < n; i += 2)
             {
-                copies_wait<D - 1>();
-                const W* s = slot(i);
-                In in;
-                in.x = s[0];
-                if constexpr (GATED) in.g = s[blockDim.x];
-                if constexpr (GRAD) in.dy = s[(kTensors - 1) * blockDim.x];
-                use(in);
-                if (i + D < n) copy(i + D);
-                copies_commit();
+                copies_wait<D / 2 - 1>();
+                W* s = slot(i);
+                const In a = get(s), b = get(s + kTensors * (int)blockDim.x);
+                use(a);
+                use(b);
+                copy(i + D, s);
+            }
+            if (i < n)
+            {
+                copies_wait<0>();
+                use(get(slot(i)));
             }
         }
         else
@@ -1075,8 +1092,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
     staged(
         n, most,
         [&](int i) {
-            copy_async<V::kBytes>(sx + i * T_, x.at(i));
-            if constexpr (GATED) copy_async<V::kBytes>(sg + i * T_, g.at(i));
+            copy_async<V::kBytes, GATED>(sx + i * T_, x.at(i));
+            if constexpr (GATED) copy_async<V::kBytes, true>(sg + i * T_, g.at(i));
         },
         [&] { stage_params(a, c0, params); },
         [&](int i) {
@@ -1182,9 +1199,9 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         staged(
             n, most,
             [&](int i) {
-                copy_async<V::kBytes>(sx + i * T_, x.at(i));
-                copy_async<V::kBytes>(sd + i * T_, d.at(i));
-                if constexpr (GATED) copy_async<V::kBytes>(sg + i * T_, g.at(i));
+                copy_async<V::kBytes, GATED>(sx + i * T_, x.at(i));
+                copy_async<V::kBytes, false>(sd + i * T_, d.at(i));
+                if constexpr (GATED) copy_async<V::kBytes, true>(sg + i * T_, g.at(i));
             },
             [&] {
                 stage_params(a, c0, params);

@@ -16,6 +16,8 @@
 #include <torch/library.h>
 #include <torch/torch.h>
 
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -531,10 +533,12 @@ static adop_norm_image norm_image(const Tensor& t, int64_t c0 = 0)
     im.data = static_cast<char*>(t.data_ptr()) + c0 * t.element_size();
     return im;
 }
+// new tensors straight from the allocator: a small image's kernels take less time than the dispatcher's way to it
 static Tensor new_image(const Tensor& like, int64_t channels)
 {
-    return torch::empty({like.size(0), channels, like.size(2), like.size(3)}, like.options().memory_format(torch::MemoryFormat::ChannelsLast));
+    return at::detail::empty_cuda({like.size(0), channels, like.size(2), like.size(3)}, like.scalar_type(), like.device(), torch::MemoryFormat::ChannelsLast);
 }
+static Tensor new_like(const Tensor& like) { return at::detail::empty_cuda(like.sizes(), like.scalar_type(), like.device(), c10::nullopt); }
 static adop_norm_params norm_params(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps, int64_t activation, bool gated)
 {
     TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
@@ -557,14 +561,20 @@ static adop_norm_params norm_params(const Tensor& x, const Tensor& weight, const
     if (bias.defined()) p.bias = bias.data_ptr();
     return p;
 }
-static Tensor norm_workspace(const adop_norm_params& p, bool gated, bool backward, const Tensor& x, adop_norm_io* io)
+// A group norm call with the workspace that it turns out to need: images that stay on the chip take none.
+using NormEntry = adop_status (*)(const adop_norm_params*, const adop_norm_io*, void*);
+static void call_group_norm(NormEntry entry, const adop_norm_params& p, adop_norm_io& io, bool backward, const char* what)
 {
-    const size_t bytes = adop_group_norm_workspace_bytes(&p, gated, backward);
-    if (bytes == 0) return Tensor();
-    Tensor ws = torch::empty({(int64_t)bytes}, x.options().dtype(torch::kUInt8).memory_format(torch::MemoryFormat::Contiguous));
-    io->workspace = ws.data_ptr();
-    io->workspace_bytes = bytes;
-    return ws;
+    void* stream = c10::cuda::getCurrentCUDAStream().stream();
+    adop_status st = entry(&p, &io, stream);
+    if (st == ADOP_ERR_WORKSPACE_TOO_SMALL)
+    {
+        io.workspace_bytes = adop_group_norm_workspace_bytes(&p, io.gate.data != nullptr, backward);
+        const at::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(io.workspace_bytes);
+        io.workspace = workspace.get();
+        st = entry(&p, &io, stream);
+    }
+    check_status(st, what);
 }
 // x in channels-last order; stats: [2,B,G] float32 for mean and rstd, or undefined
 static Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps, int64_t activation, bool gated,
@@ -582,8 +592,7 @@ static Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Te
         io.mean = stats.data_ptr<float>();
         io.rstd = io.mean + stats.numel() / 2;
     }
-    Tensor ws = norm_workspace(p, gated, false, x, &io);
-    check_status(adop_group_norm_forward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_group_norm_forward");
+    call_group_norm(adop_group_norm_forward, p, io, false, "adop_group_norm_forward");
     return y;
 }
 static bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -598,11 +607,11 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm>
                             int64_t activation, bool gated)
     {
         const Tensor weight = weight_ ? *weight_ : Tensor(), bias = bias_ ? *bias_ : Tensor();
-        Tensor stats = torch::empty({2, x.size(0), groups}, x.options().dtype(torch::kFloat32).memory_format(torch::MemoryFormat::Contiguous));
+        Tensor stats = at::detail::empty_cuda({2, x.size(0), groups}, torch::kFloat32, x.device(), c10::nullopt);
         Tensor y = group_norm_forward(x, weight, bias, groups, eps, activation, gated, stats);
         ctx->save_for_backward({x, weight, bias, stats});
-        ctx->saved_data["groups"] = groups; ctx->saved_data["eps"] = eps; ctx->saved_data["activation"] = activation;
-        ctx->saved_data["gated"] = gated;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["how"] = activation * 2 + (gated ? 1 : 0);
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grad_output)
@@ -610,9 +619,9 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm>
         once_differentiable("group_norm");
         auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
-        const bool gated = ctx->saved_data["gated"].toBool();
-        const adop_norm_params p = norm_params(x, weight, bias, ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
-                                               ctx->saved_data["activation"].toInt(), gated);
+        const int64_t how = ctx->saved_data["how"].toInt();
+        const bool gated = how % 2 != 0;
+        const adop_norm_params p = norm_params(x, weight, bias, stats.size(2), ctx->saved_data["eps"].toDouble(), how / 2, gated);
         c10::cuda::CUDAGuard guard(x.device());
         Tensor dy = channels_last(grad_output[0]), dx = new_image(x, x.size(1)), dw, db;
         adop_norm_io io{};
@@ -625,10 +634,9 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm>
             io.mean = stats.data_ptr<float>();
             io.rstd = io.mean + stats.numel() / 2;
         }
-        if (wants_gradient(weight)) { dw = torch::empty_like(weight); io.grad_weight = dw.data_ptr(); }
-        if (wants_gradient(bias)) { db = torch::empty_like(bias); io.grad_bias = db.data_ptr(); }
-        Tensor ws = norm_workspace(p, gated, true, x, &io);
-        check_status(adop_group_norm_backward(&p, &io, c10::cuda::getCurrentCUDAStream().stream()), "adop_group_norm_backward");
+        if (wants_gradient(weight)) { dw = new_like(weight); io.grad_weight = dw.data_ptr(); }
+        if (wants_gradient(bias)) { db = new_like(bias); io.grad_bias = db.data_ptr(); }
+        call_group_norm(adop_group_norm_backward, p, io, true, "adop_group_norm_backward");
         return {dx, dw, db, Variable(), Variable(), Variable(), Variable()};
     }
 };

@@ -527,8 +527,10 @@ typedef struct adop_norm_io
     size_t workspace_bytes;
 } adop_norm_io;
 
-/* Bytes of workspace that a group norm call makes use of on the current device, with or without a gate image; 0 for
- * arguments that the call refuses, and where it needs none. */
+/* Bytes of workspace that a group norm call may make use of on the current device, with or without a gate image; 0 for
+ * arguments that the call refuses, and where it needs none. A call that keeps its images on the chip needs none either, as it
+ * turns out from the tensors' addresses and strides: one that does not returns ADOP_ERR_WORKSPACE_TOO_SMALL, with nothing
+ * launched, where it is given less. */
 size_t adop_group_norm_workspace_bytes(const adop_norm_params* p, int32_t gated, int32_t backward);
 adop_status adop_group_norm_forward(const adop_norm_params* p, const adop_norm_io* io, void* stream);
 adop_status adop_group_norm_backward(const adop_norm_params* p, const adop_norm_io* io, void* stream);

@@ -88,12 +88,15 @@ def test_images(lib, entry):
 
 @pytest.mark.parametrize("backward", [0, 1])
 def test_workspace_and_statistics(lib, backward):
-    entry = ENTRIES[backward]
-    need = lib.adop_group_norm_workspace_bytes(C.byref(params()), 1, backward)
-    if need:
-        assert call(lib, entry, params(), io(workspace_bytes=need - 1)) == WORKSPACE
-        assert call(lib, entry, params(), io(workspace=None)) == WORKSPACE
-        assert call(lib, entry, params(), io(workspace=66 * P + 8)) == INVALID
+    """Images that no cluster's shared memory holds; smaller ones may need no workspace."""
+    entry, big = ENTRIES[backward], params(pixels=1 << 20)
+    stride = (1 << 20) * 16
+    images = {name: capi.AdopNormImage(P * (k + 1), stride, 16) for k, name in enumerate(("x", "gate", "y", "grad_y", "grad_x", "grad_gate"))}
+    need = lib.adop_group_norm_workspace_bytes(C.byref(big), 1, backward)
+    assert need > 0
+    assert call(lib, entry, big, io(workspace_bytes=need - 1, **images)) == WORKSPACE
+    assert call(lib, entry, big, io(workspace=None, **images)) == WORKSPACE
+    assert call(lib, entry, big, io(workspace=66 * P + 8, **images)) == INVALID
     assert call(lib, entry, params(), io(mean=None)) == INVALID
     assert call(lib, entry, params(), io(rstd=None)) == INVALID
 

@@ -61,6 +61,8 @@ adop_status check_image(const adop_norm_params* p, const adop_norm_image& im, bo
     return ADOP_OK;
 }
 
+constexpr size_t kMostShared = 220 * 1024;  // of a block
+
 // Vector and row of a call. The widest vector that every tensor's address and strides allow: 16 bytes, 8 bytes or one element.
 // A vector either lies within a pixel's channels, or all tensors are dense and a row of lcm(channels, vector) elements holds
 // whole pixels, an even number of times per image.
@@ -135,64 +137,59 @@ constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 size_t group_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->num_groups); }
 size_t channel_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->channels); }
 
-// ---- images that stay in shared memory --------------------------------------------------------------------------------------
-// A cluster of `k` blocks takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side.
-constexpr int64_t kSliceBytes = 64;
-struct Resident
-{
-    int slices, k, threads, R;  // slices: log2
-    size_t fixed, smem;  // bytes in front of the vectors, and in all
-};
 // block_sums' scratch, as the kernel lays it out
 size_t sums_scratch(const Shape& sh, int m, int R, int threads)
 {
     return sizeof(float) * 2 * (size_t)(sh.V / m) * (32 % sh.P == 0 ? threads / 32 : R) * sh.P;
 }
-bool resident_of(const adop_norm_params* p, const Shape& sh, bool gated, bool backward, Resident* r)
+
+// ---- images that stay in a block's shared memory ----------------------------------------------------------------------------
+// A block takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side. One launch in place of two
+// and no workspace: on the host it saves 4 us of 12. On the device a block of 48 KB takes 7 us whatever the others do, two launches over
+// the whole GPU 6 to 8 us; where there is a block for every other SM, 96 KB take as long as two launches do (sixteen images of 1 MB: 13.8
+// against 13.5 us).
+constexpr int64_t kSliceBytes = 64;
+#define kResidentBytes (48 << 10)
+#define kResidentManyBytes (96 << 10)
+struct Resident
+{
+    int slices, threads, R;  // slices: log2
+    size_t fixed, smem;      // bytes in front of the vectors, and in all
+};
+bool resident_of(const adop_norm_params* p, const Shape& sh, bool gated, Resident* r)
 {
     if (sh.vec == kVec1) return false;
-    const int es = element_size(p->type), tensors = 1 + (gated ? 1 : 0) + (backward ? 1 : 0), most = backward ? kNormGradThreads : kNormThreads;
-    const int64_t image = p->pixels * p->channels * es * tensors, cap = 96 << 10, least = 16 << 10;
-    const int64_t want = sm_count();
-    if (image > cap * 8 * p->num_groups) return false;
-    // the fewest blocks that hold the image; then more while there are fewer blocks than SMs and each has something to do
-    bool found = false;
-    for (int log2 = 0; log2 <= 6 && 1 << log2 <= p->num_groups; ++log2)
+    const int es = element_size(p->type), tensors = gated ? 2 : 1;
+    const int64_t rows = p->pixels / sh.ppr;
+    if (rows * sh.P * sh.V * es * tensors > kResidentManyBytes * p->num_groups) return false;
+    // the fewest ranges that do
+    for (int log2 = 0; log2 <= 12 && p->num_groups % (1 << log2) == 0; ++log2)
     {
-        const int slices = 1 << log2;
-        if (p->num_groups % slices != 0) break;
-        const int C = p->channels / slices;
-        if (slices > 1 && (sh.ppr != 1 || C % sh.V != 0 || (int64_t)C * es < kSliceBytes || (int64_t)p->batch * slices > 65535)) break;
-        const int64_t part = image / slices, rows = p->pixels / sh.ppr;
-        for (int k = 1; k <= 8 && k <= rows; k *= 2)
-        {
-            Shape s = sh;
-            s.P = sh.P / slices;
-            if (s.P > most) continue;
-            Resident c{log2, k};
-            threads_of(s.P, most, &c.R, &c.threads);
-            const int G = p->num_groups / slices, m = (int)gcd64(p->channels / p->num_groups, sh.V);
-            const int64_t here = (rows + k - 1) / k, vectors = (here + c.R - 1) / c.R * c.threads * sh.V * es * tensors;
-            if (vectors > cap) continue;
-            if (found && ((int64_t)p->batch << r->slices) * r->k >= want) return true;
-            if (found && part / k < least) return true;
-            c.fixed = sizeof(double2) * G + sizeof(float2) * 2 * G + sums_scratch(s, backward ? 1 : m, c.R, c.threads) +
-                      sizeof(float) * (2 * (size_t)C + (backward ? 2 * (size_t)C : (size_t)s.P * (sh.V / m)));
-            c.fixed = align16(c.fixed);
-            c.smem = c.fixed + (size_t)vectors;
-            if (c.smem > 200 * 1024) continue;
-            *r = c;
-            found = true;
-        }
+        const int slices = 1 << log2, C = p->channels / slices, G = p->num_groups / slices;
+        if (log2 > 0 && (sh.ppr != 1 || C % sh.V != 0 || (int64_t)C * es < kSliceBytes)) return false;
+        Shape s = sh;
+        s.P = sh.P / slices;
+        if (s.P > kNormThreads) continue;
+        Resident c{log2};
+        threads_of(s.P, kNormThreads, &c.R, &c.threads);
+        const int64_t vectors = (rows + c.R - 1) / c.R * c.threads * sh.V * es * tensors;
+        const bool many = ((int64_t)p->batch << log2) * 2 >= sm_count();
+        if (vectors > (many ? kResidentManyBytes : kResidentBytes)) continue;
+        const int m = (int)gcd64(p->channels / p->num_groups, sh.V);
+        c.fixed = align16(sizeof(float2) * G + sizeof(float) * (2 * (size_t)C + (size_t)s.P * (sh.V / m)) + sums_scratch(s, m, c.R, c.threads));
+        c.smem = c.fixed + (size_t)vectors;
+        if (c.smem > kMostShared) continue;
+        *r = c;
+        return true;
     }
-    return found;
+    return false;
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 struct Launch
 {
     const char* name;
-    int which, threads, cluster;
+    int which, threads;
     dim3 grid;
     size_t smem;
     bool early;  // may start before the launch in front of it has ended (it waits by itself)
@@ -213,28 +210,18 @@ adop_status launch(const Launch& l, const adop_norm_params* p, const Shape& sh, 
         int device = 0;
         ADOP_CUDA_TRY(cudaGetDevice(&device));
         ADOP_CUDA_TRY(once[p->type][l.which][sh.vec][gated][p->activation].run(
-            device, [&] { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024); }));
+            device, [&] { return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared); }));
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = l.grid;
     cfg.blockDim = dim3((unsigned)l.threads);
     cfg.dynamicSmemBytes = l.smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    if (l.cluster > 1)
-    {
-        cudaLaunchAttribute& c = attr[cfg.numAttrs++];
-        c.id = cudaLaunchAttributeClusterDimension;
-        c.val.clusterDim.x = (unsigned)l.cluster;
-        c.val.clusterDim.y = c.val.clusterDim.z = 1;
-    }
-    if (l.early)
-    {
-        cudaLaunchAttribute& c = attr[cfg.numAttrs++];
-        c.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        c.val.programmaticStreamSerializationAllowed = 1;
-    }
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = l.early ? 1 : 0;
     void* args[] = {&a};
     cudaError_t e = cudaSuccess;
     ADOP_LAUNCH(l.name, st, (e = cudaLaunchKernelExC(&cfg, f, args)));
@@ -310,20 +297,6 @@ adop_status check_workspace(const adop_norm_params* p, const adop_norm_io* io, b
 
 using namespace adop;
 
-namespace {
-// the launch of a resident kernel: what a slice is to it
-NormArgs slice_args(const NormArgs& whole, const Resident& r)
-{
-    NormArgs a = whole;
-    a.slices = r.slices;
-    a.C >>= r.slices; a.G >>= r.slices; a.P >>= r.slices;
-    a.R = r.R;
-    finish(&a, r.threads, r.k);
-    a.vectors = (int)r.fixed;
-    return a;
-}
-}  // namespace
-
 extern "C" size_t adop_group_norm_workspace_bytes(const adop_norm_params* p, int32_t gated, int32_t backward)
 {
     if (check_params(p, true) != ADOP_OK || p->batch == 0 || p->pixels == 0) return 0;
@@ -351,10 +324,14 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     a.mean = io->mean; a.rstd = io->rstd;
     a.group_part = static_cast<float2*>(io->workspace);
     Resident r;
-    if (resident_of(p, sh, gated, false, &r))
+    if (resident_of(p, sh, gated, &r))
     {
-        NormArgs s = slice_args(a, r);
-        return launch({"k_norm_resident", kNormResident, r.threads, r.k, dim3((unsigned)r.k, (unsigned)p->batch << r.slices), r.smem, false}, p, sh, gated, s, st);
+        a.slices = r.slices;
+        a.C >>= r.slices; a.G >>= r.slices; a.P >>= r.slices;
+        a.R = r.R;
+        finish(&a, r.threads, 1);
+        a.vectors = (int)r.fixed;
+        return launch({"k_norm_resident", kNormResident, r.threads, dim3((unsigned)p->batch << r.slices), r.smem, false}, p, sh, gated, a, st);
     }
     ADOP_TRY(check_workspace(p, io, gated, false));
     int threads;
@@ -368,10 +345,10 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     {
         const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
         a.vectors = (int)align16(smem_stats);
-        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_stats, sh, es, threads, gated, false), a.image0 > 0}, p,
+        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_stats, sh, es, threads, gated, false), a.image0 > 0}, p,
                         sh, gated, a, st));
         a.vectors = (int)align16(smem_apply);
-        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_apply, sh, es, threads, gated, false), true}, p, sh,
+        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_apply, sh, es, threads, gated, false), true}, p, sh,
                         gated, a, st));
     }
     return ADOP_OK;
@@ -402,8 +379,20 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         ADOP_TRY(check_image(p, io->grad_gate, true, "grad_gate"));
     }
     const adop_norm_image* images[5] = {&io->x, &io->grad_y, &io->grad_x, &io->gate, &io->grad_gate};
-    const Shape sh = choose_shape(p, images, gated ? 5 : 3);
-    NormArgs a = args_of(p, sh, true);
+    const int es = element_size(p->type);
+    Shape sh;
+    NormArgs a;
+    int threads;
+    size_t smem_sums;
+    // thousands of channels leave no room for wide vectors under way beside their sums
+    for (int from = kVec16;; from = sh.vec + 1)
+    {
+        sh = choose_shape(p, images, gated ? 5 : 3, from);
+        a = args_of(p, sh, true);
+        threads_of(a.P, kNormGradThreads, &a.R, &threads);
+        smem_sums = sizeof(float2) * a.G + sizeof(float) * 4 * (size_t)a.C + sums_scratch(sh, 1, a.R, threads);
+        if (sh.vec == kVec1 || stream_smem(smem_sums, sh, es, threads, gated, true) <= kMostShared) break;
+    }
     a.x = image_of(io->x, sh);
     a.gate = image_of(io->gate, sh);
     a.dy = image_of(io->grad_y, sh);
@@ -412,30 +401,13 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
     a.mean = io->mean; a.rstd = io->rstd;
     a.dweight = io->grad_weight; a.dbias = io->grad_bias;
     const bool params = io->grad_weight || io->grad_bias;
-    Resident r;
-    if (resident_of(p, sh, gated, true, &r))
-    {
-        if (params) ADOP_TRY(check_workspace(p, io, gated, true));
-        NormArgs s = slice_args(a, r);
-        s.channel_part = params ? static_cast<float2*>(io->workspace) : nullptr;
-        s.param_parts = p->batch;
-        ADOP_TRY(launch({"k_norm_grad_resident", kNormGradResident, r.threads, r.k, dim3((unsigned)r.k, (unsigned)p->batch << r.slices), r.smem, false}, p, sh,
-                        gated, s, st));
-        if (!params) return ADOP_OK;
-        return launch({"k_norm_grad_params", kNormGradParams, kNormGradThreads, 1, dim3((unsigned)((a.C + kParamChannels - 1) / kParamChannels)),
-                       sizeof(double) * 2 * kNormGradThreads, true}, p, sh, gated, s, st);
-    }
     ADOP_TRY(check_workspace(p, io, gated, true));
-    int threads;
-    threads_of(a.P, kNormGradThreads, &a.R, &threads);
     const Share share = share_of(p, gated, true);
     finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
     a.group_part = static_cast<float2*>(io->workspace);
     a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.chunks)) : nullptr;
     a.param_parts = p->batch * a.chunks;
-    const size_t smem_sums = sizeof(float2) * a.G + sizeof(float) * 4 * (size_t)a.C + sums_scratch(sh, 1, a.R, threads);
     size_t smem_apply = apply_smem(a);
-    const int es = element_size(p->type);
     if (params && smem_apply < sizeof(double) * 2 * threads) smem_apply = sizeof(double) * 2 * threads;
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
     {
@@ -443,10 +415,10 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         // the parameters' gradients need the sums of all images: blocks of the last launch add them up
         a.param_blocks = params && a.image0 + share.images >= p->batch ? (a.C + kParamChannels - 1) / kParamChannels : 0;
         a.vectors = (int)align16(smem_sums);
-        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, 1, dim3((unsigned)a.chunks, n), stream_smem(smem_sums, sh, es, threads, gated, true),
+        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_sums, sh, es, threads, gated, true),
                          a.image0 > 0}, p, sh, gated, a, st));
         a.vectors = (int)align16(smem_apply);
-        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, 1, dim3((unsigned)(a.chunks + a.param_blocks), n),
+        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, dim3((unsigned)(a.chunks + a.param_blocks), n),
                          stream_smem(smem_apply, sh, es, threads, gated, true), true}, p, sh, gated, a, st));
     }
     return ADOP_OK;
@@ -463,7 +435,7 @@ adop_status gate_launch(const adop_norm_params* p, const Shape& sh, NormArgs& a,
     if (chunks > worth) chunks = worth;
     if (chunks > a.rows) chunks = a.rows;
     finish(&a, threads, (int)chunks);
-    return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, 1, dim3((unsigned)chunks, (unsigned)p->batch), 0, false}, p, sh,
+    return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, dim3((unsigned)chunks, (unsigned)p->batch), 0, false}, p, sh,
                   true, a, st);
 }
 }  // namespace

@@ -10,7 +10,6 @@
 // None of it is a contraction: every value is read, a handful of operations are done, and it is written. HBM bounds it, and
 // for 16-bit gates the special-function unit comes close (an exponential and a reciprocal per sigmoid).
 #pragma once
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -19,8 +18,6 @@
 
 namespace adop {
 namespace norm {
-
-namespace cg = cooperative_groups;
 
 // ---- vectors ------------------------------------------------------------------------------------------------------------
 // VEC values of a vector in 32 bits, in pairs: sm_100 adds, multiplies and fuses two at a time (one instruction a pair). With one
@@ -587,19 +584,6 @@ __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part par
         if (g < a.G && lane == 0) f(g, sum);
     }
 }
-// element g of a [G] array of every block of the cluster, added up
-__device__ __forceinline__ double2 cluster_sum(cg::cluster_group& cluster, double2* own, int g)
-{
-    const int k = (int)cluster.num_blocks();
-    if (k == 1) return own[g];
-    double2 s = make_double2(0.0, 0.0);
-    for (int o = 0; o < k; ++o)
-    {
-        const double2 v = cluster.map_shared_rank(own, o)[g];
-        s.x += v.x; s.y += v.y;
-    }
-    return s;
-}
 __device__ __forceinline__ float2 mean_rstd(double2 sums, double inv_n, float eps)
 {
     const double mean = sums.x * inv_n;
@@ -681,7 +665,7 @@ template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>&
     }
 }
 
-// ---- forward, images larger than a cluster's shared memory ------------------------------------------------------------------
+// ---- forward, images larger than a block's shared memory ------------------------------------------------------------------
 // Two launches, sums and what follows, a block on each SM for either. Both take less than half an SM and may start while the launch in
 // front of them runs: the next images' sums and these images' results share the SMs, and a launch has its first vectors when its turn
 // comes.
@@ -897,21 +881,6 @@ __device__ __forceinline__ void channel_and_group_sums(const NormArgs& a, const 
         if (g < a.G && lane == 0) f(g, make_double2(s, q));
     }
 }
-// the channels' sums of the cluster's blocks, spread over its threads
-__device__ __forceinline__ void put_channels(cg::cluster_group& cluster, const NormArgs& a, float* chan, float2* out)
-{
-    const int k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    for (int c = rank * blockDim.x + threadIdx.x; c < a.C; c += k * blockDim.x)
-    {
-        float s = 0.f, q = 0.f;
-        for (int o = 0; o < k; ++o)
-        {
-            const float* p = cluster.map_shared_rank(chan, o);
-            s += p[c]; q += p[a.C + c];
-        }
-        out[c] = make_float2(s, q);
-    }
-}
 
 // Shared memory: float2 stat[G] | float params[2 C] | chan[2 C] | block_sums' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
@@ -956,9 +925,9 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
     wait_previous();
 }
 
-// db and dw of nc channels from c0 on, of `channels` in all, from the partial sums of each, in 64 bits and in a fixed order.
+// db and dw of nc channels from c0 on from the partial sums of each, in 64 bits and in a fixed order.
 // Scratch: 2 blockDim double.
-__device__ __forceinline__ void param_gradients(const NormArgs& a, int channels, int c0, int nc, double* scratch)
+__device__ __forceinline__ void param_gradients(const NormArgs& a, int c0, int nc, double* scratch)
 {
     const int T = blockDim.x, t = threadIdx.x, ways = T / nc;
     const int w = t / nc, c = t - w * nc;
@@ -967,7 +936,7 @@ __device__ __forceinline__ void param_gradients(const NormArgs& a, int channels,
 #pragma unroll 8
         for (int k = w; k < a.param_parts; k += ways)
         {
-            const float2 v = __ldcg(a.channel_part + (size_t)k * channels + c0 + c);
+            const float2 v = __ldcg(a.channel_part + (size_t)k * a.C + c0 + c);
             s += v.x; q += v.y;
         }
     scratch[2 * t] = s;
@@ -995,7 +964,7 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         if (blockIdx.y == 0)
         {
             const int c0 = blockIdx.x * kParamChannels;
-            param_gradients(a, a.C, c0, min(kParamChannels, a.C - c0), reinterpret_cast<double*>(smem));
+            param_gradients(a, c0, min(kParamChannels, a.C - c0), reinterpret_cast<double*>(smem));
         }
         return;
     }
@@ -1037,9 +1006,9 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
     }
 }
 
-// ---- images that fit a cluster's shared memory ------------------------------------------------------------------------------
-// A cluster of blocks keeps one image, or some groups' channels of it, in shared memory between the sums and what follows: every
-// value is read from global memory once. A thread copies, reads and overwrites vectors of its own only.
+// ---- images that fit a block's shared memory ----------------------------------------------------------------------------------
+// A block keeps an image, or some groups' channels of it, between the sums and what follows: one launch, every value read once. A
+// thread copies, reads and overwrites vectors of its own only.
 // n vectors in four groups: all copies are under way before the first group is used
 template <class Copy, class Between, class Use> __device__ __forceinline__ void staged(int n, int most, Copy copy, Between between, Use use)
 {
@@ -1061,39 +1030,39 @@ template <class Copy, class Between, class Use> __device__ __forceinline__ void 
     for (int i = 3 * quarter; i < n; ++i) use(i);
 }
 
-// Shared memory: double2 group[G] | float2 stat[G] | float params[2 C] | pivots[P VEC / m] | block_sums' scratch | vectors
+// Shared memory: float2 stat[G] | float params[2 C] | pivots[P VEC / m] | block_sums' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(const __grid_constant__ NormArgs a)
 {
     extern __shared__ double2 smem[];
-    auto cluster = cg::this_cluster();
-    const int t = threadIdx.x, T_ = blockDim.x, k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int b = blockIdx.y >> a.slices, slice = blockIdx.y - (b << a.slices), c0 = slice * a.C;
-    int begin, end;
-    chunk_of(a, rank, begin, end);
-    double2* group = smem;
-    float2* stat = reinterpret_cast<float2*>(group + a.G);
+    const int T_ = blockDim.x, b = blockIdx.x >> a.slices, slice = blockIdx.x - (b << a.slices), c0 = slice * a.C;
+    float2* stat = reinterpret_cast<float2*>(smem);
     float* params = reinterpret_cast<float*>(stat + a.G);
     float* shared = params + 2 * a.C;
     float* buf = shared + a.P * (VEC / a.m);
     using V = Vec<T, VEC>;
     using W = typename V::W;
     using In = Input<T, VEC>;
-    const int most = (end - begin + a.R - 1) / a.R;
-    W* sx = reinterpret_cast<W*>(reinterpret_cast<char*>(smem) + a.vectors) + t;
+    const int most = (a.rows - 1) / a.R + 1;
+    W* sx = reinterpret_cast<W*>(reinterpret_cast<char*>(smem) + a.vectors) + threadIdx.x;
     W* sg = sx + (size_t)most * T_;
     const Place pl(a, 0);
-    const int n = pl.active ? pl.count(a, begin, end) : 0;
+    const int n = pl.active ? pl.count(a, 0, a.rows) : 0;
     constexpr int H = Lanes<VEC>::N / 2;  // u in 32 bits takes the room of x and of the gate, or of x alone
     Lanes<VEC> v[2], pivot;
     v[0].fill(0.f); v[1].fill(0.f); pivot.fill(0.f);
-    const Walk<T> x(a.x, b, c0, pl, a.R, VEC, begin, end, false), g(a.gate, b, c0, pl, a.R, VEC, begin, end, false);
+    Walk<T> x(a.x, b, c0, pl, a.R, VEC, 0, a.rows, false), g(a.gate, b, c0, pl, a.R, VEC, 0, a.rows, false);
     bool have = false;
     staged(
         n, most,
         [&](int i) {
-            copy_async<V::kBytes, GATED>(sx + i * T_, x.at(i));
-            if constexpr (GATED) copy_async<V::kBytes, true>(sg + i * T_, g.at(i));
+            copy_async<V::kBytes, GATED>(sx + i * T_, x.p);
+            x.on(1);
+            if constexpr (GATED)
+            {
+                copy_async<V::kBytes, true>(sg + i * T_, g.p);
+                g.on(1);
+            }
         },
         [&] { stage_params(a, c0, params); },
         [&](int i) {
@@ -1117,135 +1086,37 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
     common_pivot<VEC>(v, pivot, n, a, pl, shared);
     block_sums<VEC>(v, a.m, a, pl, buf);
     __syncthreads();
-    group_sums<VEC>(a, end - begin, buf, shared, [&](int g, double2 sums) { group[g] = sums; });
-    if (k > 1) cluster.sync();
-    else __syncthreads();
-    const size_t g0 = (((size_t)b << a.slices) + slice) * a.G;
-    for (int i = t; i < a.G; i += T_)
-    {
-        const float2 s = mean_rstd(cluster_sum(cluster, group, i), a.inv_n, a.eps);
+    const size_t g0 = (size_t)blockIdx.x * a.G;
+    group_sums<VEC>(a, a.rows, buf, shared, [&](int i, double2 sums) {
+        const float2 s = mean_rstd(sums, a.inv_n, a.eps);
         stat[i] = s;
-        if (a.mean && rank == 0)
+        if (a.mean)
         {
             a.mean[g0 + i] = s.x;
             a.rstd[g0 + i] = s.y;
         }
-    }
+    });
     __syncthreads();
-    if (k > 1) cluster.barrier_arrive();
-    if (n > 0)
-    {
-        Forward<VEC> f;
-        f.set(a, pl.ph, stat, params);
-        const Walk<T> y(a.y, b, c0, pl, a.R, VEC, begin, end, false);
+    if (n == 0) return;
+    Forward<VEC> f;
+    f.set(a, pl.ph, stat, params);
+    Walk<T> y(a.y, b, c0, pl, a.R, VEC, 0, a.rows, false);
 #pragma unroll 2
-        for (int i = 0; i < n; ++i)
+    for (int i = 0; i < n; ++i)
+    {
+        Lanes<VEC> u;
+        const W w = sx[i * T_];
+        if constexpr (!GATED) u = V::unpack(w);
+        else if constexpr (sizeof(T) == 4) *reinterpret_cast<W*>(&u) = w;
+        else
         {
-            Lanes<VEC> u;
-            const W w = sx[i * T_];
-            if constexpr (!GATED) u = V::unpack(w);
-            else if constexpr (sizeof(T) == 4) *reinterpret_cast<W*>(&u) = w;
-            else
-            {
-                *reinterpret_cast<W*>(&u.p[0]) = w;
-                *reinterpret_cast<W*>(&u.p[H]) = sg[i * T_];
-            }
-            normalise<T, VEC, GATED, ACT>(u, f, a.act);
-            V::store(y.at(i), u);
+            *reinterpret_cast<W*>(&u.p[0]) = w;
+            *reinterpret_cast<W*>(&u.p[H]) = sg[i * T_];
         }
+        normalise<T, VEC, GATED, ACT>(u, f, a.act);
+        V::store(y.p, u);
+        y.on(1);
     }
-    if (k > 1) cluster.barrier_wait();  // nobody leaves while its sums may still be read
-}
-
-// Shared memory: double2 group[G] | float2 c12[G] | stat[G] | float params[2 C] | chan[2 C] | block_sums' scratch | vectors
-template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad_resident(const __grid_constant__ NormArgs a)
-{
-    extern __shared__ double2 smem[];
-    let_next_start();
-    auto cluster = cg::this_cluster();
-    const int t = threadIdx.x, T_ = blockDim.x, k = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int b = blockIdx.y >> a.slices, slice = blockIdx.y - (b << a.slices), c0 = slice * a.C;
-    int begin, end;
-    chunk_of(a, rank, begin, end);
-    double2* group = smem;
-    float2* c12 = reinterpret_cast<float2*>(group + a.G);
-    float2* stat = c12 + a.G;
-    float* params = reinterpret_cast<float*>(stat + a.G);
-    float* chan = params + 2 * a.C;
-    float* buf = chan + 2 * a.C;
-    using V = Vec<T, VEC>;
-    using W = typename V::W;
-    using In = Input<T, VEC>;
-    const int most = (end - begin + a.R - 1) / a.R;
-    W* sx = reinterpret_cast<W*>(reinterpret_cast<char*>(smem) + a.vectors) + t;
-    W* sd = sx + (size_t)most * T_;
-    W* sg = sd + (size_t)most * T_;
-    const Place pl(a, 0);
-    const int n = pl.active ? pl.count(a, begin, end) : 0;
-    auto get = [&](int i) {
-        In in;
-        in.x = sx[i * T_];
-        in.dy = sd[i * T_];
-        if constexpr (GATED) in.g = sg[i * T_];
-        return in;
-    };
-    Lanes<VEC> v[2];
-    v[0].fill(0.f); v[1].fill(0.f);
-    {
-        const Walk<T> x(a.x, b, c0, pl, a.R, VEC, begin, end, false), g(a.gate, b, c0, pl, a.R, VEC, begin, end, false),
-            d(a.dy, b, c0, pl, a.R, VEC, begin, end, false);
-        Saved<VEC> s;
-        staged(
-            n, most,
-            [&](int i) {
-                copy_async<V::kBytes, GATED>(sx + i * T_, x.at(i));
-                copy_async<V::kBytes, false>(sd + i * T_, d.at(i));
-                if constexpr (GATED) copy_async<V::kBytes, true>(sg + i * T_, g.at(i));
-            },
-            [&] {
-                stage_params(a, c0, params);
-                stage_stats(a, (((size_t)b << a.slices) + slice) * a.G, stat);
-                __syncthreads();
-                if (pl.active) s.set(a, pl.ph, stat, params);
-            },
-            [&](int i) { add_grad_sums<T, VEC, GATED, ACT>(get(i), s, v, a.act); });
-    }
-    block_sums<VEC>(v, 1, a, pl, buf);
-    __syncthreads();
-    channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { group[g] = sums; });
-    if (k > 1) cluster.sync();
-    else __syncthreads();
-    for (int i = t; i < a.G; i += T_)
-    {
-        const double2 s = cluster_sum(cluster, group, i);
-        c12[i] = make_float2((float)(s.x * a.inv_n), (float)(s.y * a.inv_n));
-    }
-    if (a.channel_part) put_channels(cluster, a, chan, a.channel_part + (((size_t)b << a.slices) + slice) * a.C);
-    __syncthreads();
-    if (k > 1) cluster.barrier_arrive();
-    if (n > 0)
-    {
-        Backward<VEC> c;
-        c.set(a, pl.ph, stat, c12, params);
-        const Walk<T> dx(a.dx, b, c0, pl, a.R, VEC, begin, end, false), dg(a.dgate, b, c0, pl, a.R, VEC, begin, end, false);
-        for (int i = 0; i < n; ++i)
-        {
-            Lanes<VEC> o, og;
-            input_gradient<T, VEC, GATED, ACT>(get(i), c, o, og, a.act);
-            V::store(dx.at(i), o);
-            if constexpr (GATED) V::store(dg.at(i), og);
-        }
-    }
-    if (k > 1) cluster.barrier_wait();
-}
-// the parameters' gradients behind it: [B, slices * C] partial sums. Shared memory: 2 blockDim double
-template <typename T> __global__ void __launch_bounds__(kNormGradThreads) k_norm_grad_params(const __grid_constant__ NormArgs a)
-{
-    extern __shared__ double2 smem[];
-    wait_previous();
-    const int channels = a.C << a.slices, c0 = blockIdx.x * kParamChannels;
-    param_gradients(a, channels, c0, min(kParamChannels, channels - c0), reinterpret_cast<double*>(smem));
 }
 
 // ---- the gate alone -----------------------------------------------------------------------------------------------------
@@ -1327,15 +1198,11 @@ template <typename T, int VEC, bool GATED, int ACT> const void* pick(int which)
         case kNormApply: return (const void*)k_norm_apply<T, VEC, GATED, ACT>;
         case kNormGradSums: return (const void*)k_norm_grad_sums<T, VEC, GATED, ACT>;
         case kNormGradApply: return (const void*)k_norm_grad_apply<T, VEC, GATED, ACT>;
-        case kNormGradParams: return (const void*)k_norm_grad_params<T>;
         case kGate: return (const void*)k_gate<T, VEC, true, ACT>;
         case kGateGrad: return (const void*)k_gate_grad<T, VEC, true, ACT>;
     }
     if constexpr (VEC > 1)
-    {
         if (which == kNormResident) return (const void*)k_norm_resident<T, VEC, GATED, ACT>;
-        if (which == kNormGradResident) return (const void*)k_norm_grad_resident<T, VEC, GATED, ACT>;
-    }
     return nullptr;
 }
 template <typename T, int VEC, bool GATED> const void* pick_act(int which, int act)

@@ -12,9 +12,7 @@ enum NormKernel
     kNormApply,         // y = act((u - mean) rstd w + b)
     kNormGradSums,      // per channel: sums of dz and dz uhat
     kNormGradApply,     // dx, and the parameters' gradients from the sums
-    kNormResident,      // forward pass of images that fit a cluster's shared memory
-    kNormGradResident,  // backward pass of such images
-    kNormGradParams,    // the parameters' gradients behind kNormGradResident
+    kNormResident,      // forward pass of images that fit a block's shared memory
     kGate,              // y = act(f) sigmoid(g)
     kGateGrad,          // df, dg
     kNormKernels
@@ -34,7 +32,7 @@ struct NormImage
 struct NormArgs
 {
     int C, G, Cg;     // channels and groups of a slice; channels of a group
-    int slices;       // log2 of the independent channel ranges of an image (0 but in the resident kernels)
+    int slices;       // log2 of the independent channel ranges of an image (0 but in the resident kernel)
     int P, ppr;       // vectors and pixels of a row
     int R;            // rows that a block takes at once (1 when a row has more vectors than the block threads)
     int m;            // channels of a thread's vector that share a group: gcd(Cg, VEC)
@@ -56,7 +54,7 @@ struct NormArgs
     void *dweight, *dbias;
     float *mean, *rstd;   // [B, G of all slices]
     float2* group_part;   // [B, G, chunks]
-    float2* channel_part; // [B, chunks, C] (resident: [B, 1, C of all slices])
+    float2* channel_part; // [B, chunks, C]
 };
 
 // threads of a block and resident blocks of an SM that the kernels are compiled for

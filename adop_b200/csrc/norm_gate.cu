@@ -44,14 +44,14 @@ adop_status check_params(const adop_norm_params* p, bool norm)
     return ADOP_OK;
 }
 
-constexpr int64_t kStrideLimit = (int64_t)1 << 40;  // keeps every offset below 2^63
+constexpr int64_t kExtent = (int64_t)1 << 56;  // elements from the first image to the last, and of an image
 
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 adop_status check_image(const adop_norm_params* p, const adop_norm_image& im, bool output, const char* what)
 {
     if (!im.data || !aligned(im.data, (size_t)element_size(p->type))) return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
-    if (im.image_stride < 0 || im.pixel_stride < 0 || im.image_stride > kStrideLimit || im.pixel_stride > kStrideLimit / (int64_t)65536)
+    if (im.image_stride < 0 || im.pixel_stride < 0 || im.image_stride > kExtent / p->batch || im.pixel_stride > kExtent / p->pixels)
         return refuse(ADOP_ERR_INVALID_ARGUMENT, what);
     if (output)
     {
@@ -142,11 +142,10 @@ constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 size_t group_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->num_groups); }
 size_t channel_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->channels); }
 
-// block_sums' scratch, as the kernel lays it out
-size_t sums_scratch(const Shape& sh, int m, int R, int threads)
-{
-    return sizeof(float) * 2 * (size_t)(sh.V / m) * (32 % sh.P == 0 ? threads / 32 : R) * sh.P;
-}
+// the block's sums, as the kernels lay them out: block_moments' with the counts, block_sums'
+size_t sum_rows(const Shape& sh, int R, int threads) { return (size_t)(32 % sh.P == 0 ? threads / 32 : R) * sh.P; }
+size_t moments_scratch(const Shape& sh, int m, int R, int threads) { return sizeof(float) * (2 * (sh.V / m) + 1) * sum_rows(sh, R, threads); }
+size_t sums_scratch(const Shape& sh, int R, int threads) { return sizeof(float) * 2 * sh.V * sum_rows(sh, R, threads); }
 
 // ---- images that stay in a block's shared memory ----------------------------------------------------------------------------
 // A block takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side. One launch in place of two
@@ -181,7 +180,7 @@ bool resident_of(const adop_norm_params* p, const Shape& sh, bool gated, Residen
         const bool many = ((int64_t)p->batch << log2) * 2 >= sm_count();
         if (vectors > (many ? kResidentManyBytes : kResidentBytes)) continue;
         const int m = (int)gcd64(p->channels / p->num_groups, sh.V);
-        c.fixed = align16(sizeof(float2) * G + sizeof(float) * (2 * (size_t)C + (size_t)s.P * (sh.V / m)) + sums_scratch(s, m, c.R, c.threads));
+        c.fixed = align16(sizeof(float2) * G + sizeof(float) * 2 * (size_t)C + moments_scratch(s, m, c.R, c.threads));
         c.smem = c.fixed + (size_t)vectors;
         if (c.smem > kMostShared) continue;
         *r = c;
@@ -343,7 +342,7 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     threads_of(a.P, kNormThreads, &a.R, &threads);
     const Share share = share_of(p, gated, false);
     finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
-    const size_t smem_stats = sizeof(float) * a.P * (sh.V / a.m) + sums_scratch(sh, a.m, a.R, threads);
+    const size_t smem_stats = moments_scratch(sh, a.m, a.R, threads);
     const size_t smem_apply = apply_smem(a);
     const int es = element_size(p->type);
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
@@ -395,7 +394,7 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         sh = choose_shape(p, images, gated ? 5 : 3, from);
         a = args_of(p, sh, true);
         threads_of(a.P, kNormGradThreads, &a.R, &threads);
-        smem_sums = sizeof(float2) * a.G + sizeof(float) * 4 * (size_t)a.C + sums_scratch(sh, 1, a.R, threads);
+        smem_sums = sizeof(float2) * a.G + sizeof(float) * 4 * (size_t)a.C + sums_scratch(sh, a.R, threads);
         if (sh.vec == kVec1 || stream_smem(smem_sums, sh, es, threads, gated, true) <= kMostShared) break;
     }
     a.x = image_of(io->x, sh);

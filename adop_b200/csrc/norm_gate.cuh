@@ -454,36 +454,81 @@ template <typename T, int VEC, bool GATED, int ACT> __device__ __forceinline__ L
 }
 
 // ---- sums of a block ----------------------------------------------------------------------------------------------------
-// v[k]: two sums of each of a thread's channels. Runs of m channels are added up first, then the lanes of a warp that have the same
-// channels; what is left goes to buf[(slot * rows + row) * P + ph], slot = k (VEC / m) + j / m. Returns rows. The caller waits at a
-// barrier and adds the rows up, in a fixed order: the same bits on every run. In all 2 (VEC / m) rows P floats.
+// v[k]: two sums of each of a thread's channels; what is left of them per slot, a run of m channels, goes to
+// buf[((k * (VEC / m) + j / m) * rows + row) * P + ph]. The caller waits at a barrier and adds the rows up, in a fixed order: the same
+// bits on every run. In all 2 (VEC / m) rows P floats.
 __device__ __forceinline__ int sum_rows(const NormArgs& a) { return 32 % a.P == 0 ? (int)blockDim.x >> 5 : a.R; }
-template <int VEC, int STEP>
-__device__ __forceinline__ void put_sums(Lanes<VEC> (&v)[2], const NormArgs& a, const Place& pl, float* buf)
+// the lanes of a warp that have the same channels meet where there are any; who writes, and to which row
+struct Writer
 {
-    constexpr int per = VEC / STEP;
-    const int P = a.P, rows = sum_rows(a);
-    int row = pl.r0;
-    bool writer = pl.active;
-    if (32 % P == 0)
+    int row;
+    bool here;
+    __device__ __forceinline__ Writer(const NormArgs& a, const Place& pl)
     {
-        for (int o = 16; o >= P; o >>= 1)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int j = 0; j < VEC; j += STEP) v[k].set(j, v[k].get(j) + __shfl_xor_sync(0xffffffffu, v[k].get(j), o));
-        row = threadIdx.x >> 5;
-        writer = (threadIdx.x & 31) < P;
+        const bool warps = 32 % a.P == 0;
+        row = warps ? (int)threadIdx.x >> 5 : pl.r0;
+        here = warps ? ((int)threadIdx.x & 31) < a.P : pl.active;
     }
-    if (writer)
+};
+template <int VEC, int STEP> __device__ __forceinline__ void put_slots(const Lanes<VEC> (&v)[2], const NormArgs& a, const Place& pl, float* buf)
+{
+    const Writer w(a, pl);
+    const int rows = sum_rows(a);
+    if (w.here)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int j = 0; j < VEC; j += STEP) buf[((k * per + j / STEP) * rows + row) * P + pl.ph] = v[k].get(j);
+            for (int j = 0; j < VEC; j += STEP) buf[((k * (VEC / STEP) + j / STEP) * rows + w.row) * a.P + pl.ph] = v[k].get(j);
+}
+template <int VEC> __device__ __forceinline__ void block_sums(Lanes<VEC> (&v)[2], const NormArgs& a, const Place& pl, float* buf)
+{
+    if (32 % a.P == 0)
+        for (int o = 16; o >= a.P; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) v[k].set(j, v[k].get(j) + __shfl_xor_sync(0xffffffffu, v[k].get(j), o));
+    put_slots<VEC, 1>(v, a, pl, buf);
+}
+
+// Moments instead: v holds the sums of u - p and of its square over n rows, p (as its negative) one of the values. A thread's mean and sum
+// of squares about it, joined by lanes with d^2 n_a n_b / (n_a + n_b) for means d apart, so nothing cancels wherever the values lie;
+// counts[row * P + ph] gets the rows that a row of buf stands for.
+template <int VEC, int STEP>
+__device__ __forceinline__ void put_moments_of(Lanes<VEC> (&v)[2], const Lanes<VEC>& pivot, int n, const NormArgs& a, const Place& pl, float* buf, float* counts)
+{
+    float cnt = (float)n;
+    const float inv = n > 0 ? __fdividef(1.f, cnt * STEP) : 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; j += STEP)
+    {
+        const float s = v[0].get(j), d = s * inv;
+        v[1].set(j, fmaf(-s, d, v[1].get(j)));
+        v[0].set(j, d - pivot.get(j));
+    }
+    if (32 % a.P == 0)
+        for (int o = 16; o >= a.P; o >>= 1)
+        {
+            const float other = __shfl_xor_sync(0xffffffffu, cnt, o), both = cnt + other;
+            const float w = both > 0.f ? __fdividef(other, both) : 0.f, shared = cnt * w * STEP;
+#pragma unroll
+            for (int j = 0; j < VEC; j += STEP)
+            {
+                const float d = __shfl_xor_sync(0xffffffffu, v[0].get(j), o) - v[0].get(j);
+                const float q = __shfl_xor_sync(0xffffffffu, v[1].get(j), o);
+                v[1].set(j, v[1].get(j) + q + d * d * shared);
+                v[0].set(j, fmaf(d, w, v[0].get(j)));
+            }
+            cnt = both;
+        }
+    put_slots<VEC, STEP>(v, a, pl, buf);
+    const Writer w(a, pl);
+    if (w.here) counts[w.row * a.P + pl.ph] = cnt;
 }
 template <int VEC>
-__device__ __forceinline__ void block_sums(Lanes<VEC> (&v)[2], int m, const NormArgs& a, const Place& pl, float* buf)
+__device__ __forceinline__ void block_moments(Lanes<VEC> (&v)[2], const Lanes<VEC>& pivot, int n, const NormArgs& a, const Place& pl, float* buf, float* counts)
 {
+    const int m = a.m;
     if (VEC > 1 && m > 1)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -499,57 +544,41 @@ __device__ __forceinline__ void block_sums(Lanes<VEC> (&v)[2], int m, const Norm
         {
 #pragma unroll
             for (int k = 0; k < 2; ++k) v[k].p[0].x += v[k].p[2].x;
-            return put_sums<VEC, 8>(v, a, pl, buf);
+            return put_moments_of<VEC, 8>(v, pivot, n, a, pl, buf, counts);
         }
     if constexpr (VEC > 2)
-        if (m == 4) return put_sums<VEC, 4>(v, a, pl, buf);
+        if (m == 4) return put_moments_of<VEC, 4>(v, pivot, n, a, pl, buf, counts);
     if constexpr (VEC > 1)
-        if (m == 2) return put_sums<VEC, 2>(v, a, pl, buf);
-    put_sums<VEC, 1>(v, a, pl, buf);
+        if (m == 2) return put_moments_of<VEC, 2>(v, pivot, n, a, pl, buf, counts);
+    put_moments_of<VEC, 1>(v, pivot, n, a, pl, buf, counts);
 }
 
-// The block's sums of u and u^2 of a group in 64 bits, for f(g, sums), from the slots' sums of u - pivot and its square over `n` rows
-// of the image. The pivots are values of the data themselves, so the squares cancel by the number of values at most.
-template <int VEC, class F>
-__device__ __forceinline__ void group_sums(const NormArgs& a, int n, const float* buf, const float* pivot, F f)
+// The block's sums of u and u^2 of a group in 64 bits, for f(g, sums), from what block_moments left.
+template <int VEC, class F> __device__ __forceinline__ void group_sums(const NormArgs& a, const float* buf, const float* counts, F f)
 {
     const int sh = __ffs(a.m) - 1, per = VEC >> sh, run = a.Cg >> sh, slots = run * a.ppr, rows = sum_rows(a), second = per * rows * a.P;
     const int lanes = 1 << a.lanes, row_lanes = 1 << a.row_lanes, want = ((a.G << a.lanes) + 31) & ~31;
-    const double cnt = (double)n * (double)a.m;
     for (int idx = threadIdx.x; idx < want; idx += blockDim.x)
     {
+        // a group's lanes: row_lanes for a slot's rows, so many slots at a time
         const int g = idx >> a.lanes, lane = idx & (lanes - 1), row = lane & (row_lanes - 1);
         double s = 0.0, q = 0.0;
-        // a group's lanes: row_lanes for a slot's rows, so many slots at a time; the same number of turns for all of them
-        for (int slot0 = 0; slot0 < slots; slot0 += lanes >> a.row_lanes)
-        {
-            const int slot = slot0 + (lane >> a.row_lanes);
-            const bool here = g < a.G && slot < slots;
-            float ds = 0.f, dq = 0.f;
-            double piv = 0.0;
-            if (here)
+        if (g < a.G)
+            for (int slot = lane >> a.row_lanes; slot < slots; slot += lanes >> a.row_lanes)
             {
                 int i = slot, e = g * a.Cg;
                 while (i >= run) { i -= run; e += a.C; }
                 e += i << sh;
-                const int jj = (e % VEC) >> sh, p = e / VEC;
-                piv = (double)pivot[jj * a.P + p];
-                const float* col = buf + jj * rows * a.P + p;
-                for (int r = row; r < rows; r += row_lanes) { ds += col[r * a.P]; dq += col[second + r * a.P]; }
+                const int p = e / VEC;
+                const float* col = buf + ((e % VEC) >> sh) * rows * a.P + p;
+                for (int r = row; r < rows; r += row_lanes)
+                {
+                    const double mean = (double)col[r * a.P], sum = (double)(counts[r * a.P + p] * (float)a.m) * mean;
+                    s += sum;
+                    q += fma(sum, mean, (double)col[second + r * a.P]);
+                }
             }
-            for (int o = row_lanes >> 1; o > 0; o >>= 1)
-            {
-                ds += __shfl_xor_sync(0xffffffffu, ds, o);
-                dq += __shfl_xor_sync(0xffffffffu, dq, o);
-            }
-            if (here)
-            {
-                const double d = (double)ds;
-                s += fma(cnt, piv, d);
-                q += fma(piv, fma(cnt, piv, 2.0 * d), (double)dq);
-            }
-        }
-        for (int o = lanes >> 1; o >= row_lanes; o >>= 1)
+        for (int o = lanes >> 1; o > 0; o >>= 1)
         {
             s += __shfl_xor_sync(0xffffffffu, s, o);
             q += __shfl_xor_sync(0xffffffffu, q, o);
@@ -628,32 +657,6 @@ template <int VEC> __device__ __forceinline__ Lanes<VEC> pivot_of(const Lanes<VE
     for (int j = 0; j < VEC; ++j) p.set(j, (j & (m - 1)) ? p.get(j - 1) : -u.get(j));
     return p;
 }
-// A thread's sums are about its own first value: turned to that of the block's first row, which `shared` gets, n values a channel each.
-// One barrier.
-template <int VEC>
-__device__ __forceinline__ void common_pivot(Lanes<VEC> (&v)[2], const Lanes<VEC>& own, int n, const NormArgs& a, const Place& pl, float* shared)
-{
-    const int sh = __ffs(a.m) - 1;
-    if (pl.active && pl.r0 == 0)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if ((j & (a.m - 1)) == 0) shared[(j >> sh) * a.P + pl.ph] = -own.get(j);
-    __syncthreads();
-    if (n > 0 && pl.r0 > 0)
-    {
-        const float2 cnt = pair((float)n);
-#pragma unroll
-        for (int k = 0; k < Lanes<VEC>::N; ++k)
-        {
-            float2 d;
-            d.x = -own.p[k].x - shared[(2 * k >> sh) * a.P + pl.ph];
-            d.y = VEC > 1 ? -own.p[k].y - shared[((2 * k + 1) >> sh) * a.P + pl.ph] : d.x;
-            const float2 nd = mul(cnt, d);
-            v[1].p[k] = add(v[1].p[k], mul(d, add(add(v[0].p[k], v[0].p[k]), nd)));
-            v[0].p[k] = add(v[0].p[k], nd);
-        }
-    }
-}
 template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>& u, const Lanes<VEC>& pivot, Lanes<VEC> (&v)[2])
 {
 #pragma unroll
@@ -669,7 +672,7 @@ template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>&
 // Two launches, sums and what follows, a block on each SM for either. Both take less than half an SM and may start while the launch in
 // front of them runs: the next images' sums and these images' results share the SMs, and a launch has its first vectors when its turn
 // comes.
-// Shared memory: float pivots[P VEC / m] | block_sums' scratch | vectors
+// Shared memory: block_moments' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const __grid_constant__ NormArgs a)
 {
@@ -678,8 +681,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
     const int b = a.image0 + blockIdx.y;
     int begin, end;
     chunk_of(a, blockIdx.x, begin, end);
-    float* shared = reinterpret_cast<float*>(smem);
-    float* buf = shared + a.P * (VEC / a.m);
+    float* buf = reinterpret_cast<float*>(smem);
+    float* counts = buf + 2 * (VEC / a.m) * sum_rows(a) * a.P;
     for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
         const Place pl(a, ph0);
@@ -694,13 +697,12 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
             have = true;
             add_moments<VEC>(u, pivot, v);
         });
-        common_pivot<VEC>(v, pivot, in.n, a, pl, shared);
-        block_sums<VEC>(v, a.m, a, pl, buf);
+        block_moments<VEC>(v, pivot, in.n, a, pl, buf, counts);
     }
     __syncthreads();
     float2* out = a.group_part + (size_t)b * a.chunks * a.G + blockIdx.x;
     const double inv_n = (int)blockIdx.x < a.chunk_more ? a.inv_long : a.inv_short;
-    group_sums<VEC>(a, end - begin, buf, shared, [&](int g, double2 sums) {
+    group_sums<VEC>(a, buf, counts, [&](int g, double2 sums) {
         // the chunk's mean and sum of squares about it: 32 bits hold these
         const double mean = sums.x * inv_n;
         out[(size_t)g * a.chunks] = make_float2((float)mean, (float)fma(-mean, sums.x, sums.y));
@@ -914,7 +916,7 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
             s.set(a, pl.ph, stat, params);
             in.run([&](const Input<T, VEC>& i) { add_grad_sums<T, VEC, GATED, ACT>(i, s, v, a.act); });
         }
-        block_sums<VEC>(v, 1, a, pl, buf);
+        block_sums<VEC>(v, a, pl, buf);
     }
     __syncthreads();
     const size_t part = (size_t)b * a.chunks + blockIdx.x;
@@ -1030,7 +1032,7 @@ template <class Copy, class Between, class Use> __device__ __forceinline__ void 
     for (int i = 3 * quarter; i < n; ++i) use(i);
 }
 
-// Shared memory: float2 stat[G] | float params[2 C] | pivots[P VEC / m] | block_sums' scratch | vectors
+// Shared memory: float2 stat[G] | float params[2 C] | block_moments' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(const __grid_constant__ NormArgs a)
 {
@@ -1038,8 +1040,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
     const int T_ = blockDim.x, b = blockIdx.x >> a.slices, slice = blockIdx.x - (b << a.slices), c0 = slice * a.C;
     float2* stat = reinterpret_cast<float2*>(smem);
     float* params = reinterpret_cast<float*>(stat + a.G);
-    float* shared = params + 2 * a.C;
-    float* buf = shared + a.P * (VEC / a.m);
+    float* buf = params + 2 * a.C;
+    float* counts = buf + 2 * (VEC / a.m) * sum_rows(a) * a.P;
     using V = Vec<T, VEC>;
     using W = typename V::W;
     using In = Input<T, VEC>;
@@ -1083,11 +1085,10 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
                 }
             }
         });
-    common_pivot<VEC>(v, pivot, n, a, pl, shared);
-    block_sums<VEC>(v, a.m, a, pl, buf);
+    block_moments<VEC>(v, pivot, n, a, pl, buf, counts);
     __syncthreads();
     const size_t g0 = (size_t)blockIdx.x * a.G;
-    group_sums<VEC>(a, a.rows, buf, shared, [&](int i, double2 sums) {
+    group_sums<VEC>(a, buf, counts, [&](int i, double2 sums) {
         const float2 s = mean_rstd(sums, a.inv_n, a.eps);
         stat[i] = s;
         if (a.mean)

@@ -78,8 +78,8 @@ def test_images(lib, entry):
         assert call(lib, entry, params(), image(P + 1, 960, 16)) == INVALID, name      # not aligned to its type
         assert call(lib, entry, params(), image(P, -960, 16)) == INVALID, name
         assert call(lib, entry, params(), image(P, 960, -16)) == INVALID, name
-        assert call(lib, entry, params(), image(P, 1 << 41, 16)) == INVALID, name
-        assert call(lib, entry, params(), image(P, 960, 1 << 25)) == INVALID, name
+        assert call(lib, entry, params(), image(P, 1 << 56, 16)) == INVALID, name
+        assert call(lib, entry, params(), image(P, 960, 1 << 51)) == INVALID, name
         if name in ("y", "grad_x", "grad_gate"):  # the pixels of an output do not overlap
             assert call(lib, entry, params(), image(P, 960, 15)) == INVALID, name
             assert call(lib, entry, params(), image(P, 959, 16)) == INVALID, name

@@ -100,6 +100,10 @@ void threads_of(int P, int most, int* R, int* threads)
     *threads = P > most ? most : (*R * P + 31) / 32 * 32;
 }
 
+// The last launch of a backward pass shares the SMs with no other: it gets two blocks an SM where they have something to do (four images
+// of 33 MB of inputs: 77.8 -> 67.6 us; with the others' launches doubled too, sixteen of them 261 -> 290 us; parts of 35 KB 17.7 -> 19.6 us).
+constexpr int64_t kAlonePart = 64 << 10;  // bytes of one tensor
+
 // Images whose inputs are read twice, by the sums and by what follows, are taken in groups of which the L2 keeps a good part. A group
 // costs two launches (5 us of waits and tails), so two images go together up to the larger bound. Measured: four images of 33 MB of
 // inputs, backward, two by two 78 us, all at once 82 us; sixteen of 50 MB one by one 418 us, two by two 378 us.
@@ -250,6 +254,11 @@ NormArgs args_of(const adop_norm_params* p, const Shape& sh, bool norm)
     a.weight = p->weight; a.bias = p->bias;
     return a;
 }
+NormParts parts_of(int rows, int64_t count)
+{
+    if (count > rows) count = rows;
+    return {(int)count, rows / (int)count, rows % (int)count};
+}
 // what follows from the sizes of a slice, the threads and the number of parts of an image
 void finish(NormArgs* a, int threads, int chunks)
 {
@@ -261,13 +270,11 @@ void finish(NormArgs* a, int threads, int chunks)
     const int rows = 32 % a->P == 0 ? threads / 32 : a->R;
     a->row_lanes = log2_of(rows);
     a->lanes = log2_of((int64_t)(1 << a->row_lanes) * (a->Cg / a->m * a->ppr));
-    a->chunks = chunks;
-    a->chunk_rows = a->rows / chunks;
-    a->chunk_more = a->rows % chunks;
+        a->sums = a->own = parts_of(a->rows, chunks);
     const double per_row = (double)a->ppr * a->Cg;
     a->inv_n = 1.0 / (a->rows * per_row);
-    a->inv_short = 1.0 / (a->chunk_rows * per_row);
-    a->inv_long = 1.0 / ((a->chunk_rows + 1) * per_row);
+    a->inv_short = 1.0 / (a->sums.rows * per_row);
+    a->inv_long = 1.0 / ((a->sums.rows + 1) * per_row);
     a->inv_P = 1.f / a->P; a->inv_Cg = 1.f / a->Cg;
     a->gather = log2_of(chunks);
     while (a->gather > 0 && a->G << a->gather > threads) --a->gather;
@@ -349,10 +356,12 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     {
         const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
         a.vectors = (int)align16(smem_stats);
-        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_stats, sh, es, threads, gated, false), a.image0 > 0}, p,
+        a.own = a.sums;
+        ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, dim3((unsigned)a.sums.count, n), stream_smem(smem_stats, sh, es, threads, gated, false), a.image0 > 0}, p,
                         sh, gated, a, st));
         a.vectors = (int)align16(smem_apply);
-        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_apply, sh, es, threads, gated, false), true}, p, sh,
+        a.own = a.sums;
+        ADOP_TRY(launch({"k_norm_apply", kNormApply, threads, dim3((unsigned)a.own.count, n), stream_smem(smem_apply, sh, es, threads, gated, false), true}, p, sh,
                         gated, a, st));
     }
     return ADOP_OK;
@@ -409,20 +418,24 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
     const Share share = share_of(p, gated, true);
     finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
     a.group_part = static_cast<float2*>(io->workspace);
-    a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.chunks)) : nullptr;
-    a.param_parts = p->batch * a.chunks;
+    a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.sums.count)) : nullptr;
+    a.param_parts = p->batch * a.sums.count;
     size_t smem_apply = apply_smem(a);
     if (params && smem_apply < sizeof(double) * 2 * threads) smem_apply = sizeof(double) * 2 * threads;
+    const int64_t part = (int64_t)a.rows / a.sums.count * a.P * sh.V * es;
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)
     {
         const unsigned n = (unsigned)(p->batch - a.image0 < share.images ? p->batch - a.image0 : share.images);
+        const bool last = a.image0 + share.images >= p->batch;
         // the parameters' gradients need the sums of all images: blocks of the last launch add them up
-        a.param_blocks = params && a.image0 + share.images >= p->batch ? param_blocks_of(p) : 0;
+        a.param_blocks = params && last ? param_blocks_of(p) : 0;
         a.vectors = (int)align16(smem_sums);
-        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, dim3((unsigned)a.chunks, n), stream_smem(smem_sums, sh, es, threads, gated, true),
+        a.own = a.sums;
+        ADOP_TRY(launch({"k_norm_grad_sums", kNormGradSums, threads, dim3((unsigned)a.sums.count, n), stream_smem(smem_sums, sh, es, threads, gated, true),
                          a.image0 > 0}, p, sh, gated, a, st));
         a.vectors = (int)align16(smem_apply);
-        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, dim3((unsigned)(a.chunks + a.param_blocks), n),
+        a.own = last && part >= kAlonePart ? parts_of(a.rows, (int64_t)a.sums.count * 2) : a.sums;
+        ADOP_TRY(launch({"k_norm_grad_apply", kNormGradApply, threads, dim3((unsigned)(a.own.count + a.param_blocks), n),
                          stream_smem(smem_apply, sh, es, threads, gated, true), true}, p, sh, gated, a, st));
     }
     return ADOP_OK;

@@ -304,11 +304,11 @@ template <int U, class Load, class Use, class Next> __device__ __forceinline__ v
             if (i + k < n) use(k, in[k]);
     }
 }
-// rows [begin, end) of a part of the image: of the parts, the first chunk_more have a row more than the others
+// rows [begin, end) of a block's part of the image
 __device__ __forceinline__ void chunk_of(const NormArgs& a, int part, int& begin, int& end)
 {
-    begin = part * a.chunk_rows + min(part, a.chunk_more);
-    end = begin + a.chunk_rows + (part < a.chunk_more ? 1 : 0);
+    begin = part * a.own.rows + min(part, a.own.more);
+    end = begin + a.own.rows + (part < a.own.more ? 1 : 0);
 }
 // f(j, c, g) for the channels c and groups g of a thread's vector (a row of several pixels goes through the channels again)
 template <int VEC, class F> __device__ __forceinline__ void for_channels(const NormArgs& a, int ph, F f)
@@ -592,7 +592,7 @@ template <int VEC, class F> __device__ __forceinline__ void group_sums(const Nor
 template <class Part, class F>
 __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part part, F f)
 {
-    const float2* __restrict__ from = a.group_part + (size_t)b * a.chunks * a.G;
+    const float2* __restrict__ from = a.group_part + (size_t)b * a.sums.count * a.G;
     const int lanes = 1 << a.gather, want = ((a.G << a.gather) + 31) & ~31;
     for (int idx = threadIdx.x; idx < want; idx += blockDim.x)
     {
@@ -600,9 +600,9 @@ __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part par
         double2 sum = make_double2(0.0, 0.0);
         if (g < a.G)
 #pragma unroll 8
-            for (int k = lane; k < a.chunks; k += lanes)
+            for (int k = lane; k < a.sums.count; k += lanes)
             {
-                const double2 v = part(k, __ldcg(from + (size_t)g * a.chunks + k));
+                const double2 v = part(k, __ldcg(from + (size_t)g * a.sums.count + k));
                 sum.x += v.x; sum.y += v.y;
             }
         for (int o = lanes >> 1; o > 0; o >>= 1)
@@ -700,12 +700,12 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
         block_moments<VEC>(v, pivot, in.n, a, pl, buf, counts);
     }
     __syncthreads();
-    float2* out = a.group_part + (size_t)b * a.chunks * a.G + blockIdx.x;
-    const double inv_n = (int)blockIdx.x < a.chunk_more ? a.inv_long : a.inv_short;
+    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + blockIdx.x;
+    const double inv_n = (int)blockIdx.x < a.sums.more ? a.inv_long : a.inv_short;
     group_sums<VEC>(a, buf, counts, [&](int g, double2 sums) {
         // the chunk's mean and sum of squares about it: 32 bits hold these
         const double mean = sums.x * inv_n;
-        out[(size_t)g * a.chunks] = make_float2((float)mean, (float)fma(-mean, sums.x, sums.y));
+        out[(size_t)g * a.sums.count] = make_float2((float)mean, (float)fma(-mean, sums.x, sums.y));
     });
     wait_previous();
 }
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_apply(const 
             gather_groups(
                 a, b,
                 [&](int k, float2 v) {
-                    const double mean = v.x, s = (double)(a.chunk_rows + (k < a.chunk_more ? 1 : 0)) * per_row * mean;
+                    const double mean = v.x, s = (double)(a.sums.rows + (k < a.sums.more ? 1 : 0)) * per_row * mean;
                     return make_double2(s, fma(s, mean, (double)v.y));
                 },
                 [&](int g, double2 sums) {
@@ -919,9 +919,9 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         block_sums<VEC>(v, a, pl, buf);
     }
     __syncthreads();
-    const size_t part = (size_t)b * a.chunks + blockIdx.x;
-    float2* out = a.group_part + (size_t)b * a.chunks * a.G + blockIdx.x;
-    channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { out[(size_t)g * a.chunks] = make_float2((float)sums.x, (float)sums.y); });
+    const size_t part = (size_t)b * a.sums.count + blockIdx.x;
+    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + blockIdx.x;
+    channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { out[(size_t)g * a.sums.count] = make_float2((float)sums.x, (float)sums.y); });
     if (a.channel_part)
         for (int c = threadIdx.x; c < a.C; c += blockDim.x) a.channel_part[part * a.C + c] = make_float2(chan[c], chan[a.C + c]);
     wait_previous();

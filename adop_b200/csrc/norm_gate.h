@@ -27,6 +27,12 @@ struct NormImage
     int64_t image, row;
 };
 
+// An image's rows in parts: `rows` each, the first `more` of them one more.
+struct NormParts
+{
+    int count, rows, more;
+};
+
 // An image is walked in rows of P vectors: P vectors of VEC elements are the smallest run that starts and ends with a pixel,
 // so a thread that moves on by whole rows keeps its channels, and with them its coefficients and its sums, in registers.
 struct NormArgs
@@ -39,8 +45,8 @@ struct NormArgs
     int lanes, row_lanes;  // log2 of the threads that add up one group's sums, and of those for one slot's rows
     int rows;         // rows of an image
     int image0;       // first image of the launch
-    int chunks;       // parts of an image, which have a partial sum each
-    int chunk_rows, chunk_more;            // rows of a part; the first chunk_more parts have one more
+    NormParts sums;   // parts of an image that have a partial sum each
+    NormParts own;    // parts that the blocks of the launch take
     double inv_n, inv_short, inv_long;     // 1 / values of a group in the image, in a part, in one with a row more
     int gather;           // log2 of the threads that add up a group's partial sums
     float inv_P, inv_Cg;

@@ -1,6 +1,6 @@
 """Run one of the benchmark configurations end to end on one GPU and print its timings as one JSON line.
 
-    python -m adop_b200.run_config c1|c2|c3|c4|c5|reorder|tonemap [--points N] [--views V] [--reps R]
+    python -m adop_b200.run_config c1|c2|c3|c4|c5|reorder|tonemap|network [--points N] [--views V] [--reps R]
 
 bench.py measures the headline configuration (c2) under the driver's contract; this runner covers the others:
 c1 (small cloud, 512x512), c3 (100 M points, omnidirectional camera, forward only, ms per frame), c4 (30 M points, 8 views),
@@ -113,9 +113,45 @@ def tonemap(dev, args):
     return 0
 
 
+def network(dev, args):
+    """The rendering network's operators (adop::group_norm, gated_activation, gated_group_norm) at the levels of a 1080p pyramid in
+    bfloat16, 16 channels at the finest level and twice as many at each next one: time per call, forward and backward, and the
+    fraction of the HBM roofline (inputs read once, outputs written once)."""
+    from . import build
+    torch.ops.load_library(build.TORCH_OP_LIB)
+    ops = torch.ops.adop
+    peak = 6542.7
+    batch = args.views or 1
+    out = {"config": "network", "image": [1920, 1080], "batch": batch, "dtype": "bf16"}
+    g = torch.Generator(device=dev)
+    g.manual_seed(0)
+    for level, (w, h) in enumerate(capi.layer_sizes(1920, 1080, 4)):
+        c = 16 << level
+        x2 = torch.randn((batch, h, w, 2 * c), device=dev, generator=g).bfloat16().permute(0, 3, 1, 2)
+        dy = torch.randn((batch, h, w, c), device=dev, generator=g).bfloat16().permute(0, 3, 1, 2)
+        x1 = dy.clone(memory_format=torch.preserve_format).requires_grad_(True)
+        x2.requires_grad_(True)
+        weight, bias = torch.ones(c, device=dev, requires_grad=True), torch.zeros(c, device=dev, requires_grad=True)
+        calls = {"group_norm": (2, lambda: ops.group_norm(x1, 4, weight, bias, 1e-5, "silu"), [x1, weight, bias]),
+                 "gated_activation": (3, lambda: ops.gated_activation(x2, "elu"), [x2]),
+                 "gated_group_norm": (3, lambda: ops.gated_group_norm(x2, 4, weight, bias, 1e-5, "elu"), [x2, weight, bias])}
+        for name, (tensors, call, leaves) in calls.items():
+            y = call()
+            backward = lambda: torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            value_bytes = 2 * batch * h * w * c
+            for label, f, n in (("fwd", call, tensors), ("bwd", backward, 2 * tensors - 1)):
+                for _ in range(3):
+                    f()
+                t = statistics.median(timed(f, max(args.reps, 20)))
+                out[f"{name}_{w}x{h}x{c}_{label}_us"] = t * 1e3
+                out[f"{name}_{w}x{h}x{c}_{label}_frac"] = n * value_bytes / (t * 1e-3) / 1e9 / peak
+    print(json.dumps(out), flush=True)
+    return 0
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("config", choices=["c1", "c2", "c3", "c4", "c5", "reorder", "tonemap"])
+    ap.add_argument("config", choices=["c1", "c2", "c3", "c4", "c5", "reorder", "tonemap", "network"])
     ap.add_argument("--points", type=int, default=None)
     ap.add_argument("--views", type=int, default=None)
     ap.add_argument("--reps", type=int, default=5)
@@ -127,6 +163,8 @@ def main():
         return reorder(dev, args)
     if args.config == "tonemap":
         return tonemap(dev, args)
+    if args.config == "network":
+        return network(dev, args)
     cfg = synth.make_config(args.config, n_points=args.points, n_views=args.views)
     meta, params, L = cfg["meta"], cfg["params"], cfg["num_layers"]
     forward_only = args.config == "c3"

@@ -444,15 +444,16 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
 namespace {
 adop_status gate_launch(const adop_norm_params* p, const Shape& sh, NormArgs& a, bool backward, cudaStream_t st)
 {
-    const int most = backward ? kGateGradThreads : kGateThreads;
+    const int most = backward ? kNormGradThreads : kNormThreads;
     int threads;
     threads_of(a.P, most, &a.R, &threads);
     const int64_t worth = (p->pixels * p->channels * element_size(p->type) + kMinChunk - 1) / kMinChunk;
-    int64_t chunks = ((int64_t)sm_count() * kGateBlocks + p->batch - 1) / p->batch;
+    int64_t chunks = ((int64_t)sm_count() * (backward ? kNormGradBlocks : kNormBlocks) + p->batch - 1) / p->batch;
     if (chunks > worth) chunks = worth;
     if (chunks > a.rows) chunks = a.rows;
     finish(&a, threads, (int)chunks);
-    return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, dim3((unsigned)chunks, (unsigned)p->batch), 0, false}, p, sh,
+    return launch({backward ? "k_gate_grad" : "k_gate", backward ? kGateGrad : kGate, threads, dim3((unsigned)chunks, (unsigned)p->batch),
+                   stream_smem(0, sh, element_size(p->type), threads, true, backward), false}, p, sh,
                   true, a, st);
 }
 }  // namespace

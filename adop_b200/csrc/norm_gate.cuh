@@ -280,30 +280,6 @@ template <typename T> struct Walk
     __device__ __forceinline__ T* at(int k) const { return p + k * step; }
     __device__ __forceinline__ void on(int k) { p += k * step; }
 };
-// U loads are under way before the first is used
-template <int U, class Load, class Use, class Next> __device__ __forceinline__ void batches(int n, Load load, Use use, Next next)
-{
-    int i = 0;
-    for (; i + U <= n; i += U)
-    {
-        decltype(load(0)) in[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) in[k] = load(k);
-#pragma unroll
-        for (int k = 0; k < U; ++k) use(k, in[k]);
-        next(U);
-    }
-    if (U > 1 && i < n)
-    {
-        decltype(load(0)) in[U];
-#pragma unroll
-        for (int k = 0; k < U - 1; ++k)
-            if (i + k < n) in[k] = load(k);
-#pragma unroll
-        for (int k = 0; k < U - 1; ++k)
-            if (i + k < n) use(k, in[k]);
-    }
-}
 // rows [begin, end) of a block's part of the image
 __device__ __forceinline__ void chunk_of(const NormArgs& a, int part, int& begin, int& end)
 {
@@ -1121,72 +1097,56 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
 }
 
 // ---- the gate alone -----------------------------------------------------------------------------------------------------
+// Shared memory: vectors
 template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kGateThreads, kGateBlocks) k_gate(const __grid_constant__ NormArgs a)
+__global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_gate(const __grid_constant__ NormArgs a)
 {
+    extern __shared__ double2 smem[];
     const int b = blockIdx.y;
     int begin, end;
     chunk_of(a, blockIdx.x, begin, end);
-    constexpr int U = 2;
-    using V = Vec<T, VEC>;
-    using In = Input<T, VEC>;
     for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
         const Place pl(a, ph0);
-        if (!pl.active) continue;
-        Walk<T> x(a.x, b, 0, pl, a.R, VEC, begin, end, false), g(a.gate, b, 0, pl, a.R, VEC, begin, end, false), y(a.y, b, 0, pl, a.R, VEC, begin, end, false);
-        batches<U>(
-            pl.count(a, begin, end),
-            [&](int k) {
-                In i;
-                i.x = V::load(x.at(k));
-                i.g = V::load(g.at(k));
-                return i;
-            },
-            [&](int k, const In& i) { V::store(y.at(k), value_of<T, VEC, true, ACT>(i, a.act)); },
-            [&](int k) { x.on(k); g.on(k); y.on(k); });
+        Stream<T, VEC, true, false> in(a, b, pl, begin, end, false, smem);
+        in.start();
+        Walk<T> y(a.y, b, 0, pl, a.R, VEC, begin, end, false);
+        in.run([&](const Input<T, VEC>& i) {
+            Vec<T, VEC>::store(y.p, value_of<T, VEC, true, ACT>(i, a.act));
+            y.on(1);
+        });
     }
 }
 template <typename T, int VEC, bool GATED, int ACT>
-__global__ void __launch_bounds__(kGateGradThreads, kGateBlocks) k_gate_grad(const __grid_constant__ NormArgs a)
+__global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_gate_grad(const __grid_constant__ NormArgs a)
 {
+    extern __shared__ double2 smem[];
     const int b = blockIdx.y;
     int begin, end;
     chunk_of(a, blockIdx.x, begin, end);
-    constexpr int U = 2;
     using V = Vec<T, VEC>;
-    using In = Input<T, VEC>;
     for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
         const Place pl(a, ph0);
-        if (!pl.active) continue;
-        Walk<T> x(a.x, b, 0, pl, a.R, VEC, begin, end, false), g(a.gate, b, 0, pl, a.R, VEC, begin, end, false), d(a.dy, b, 0, pl, a.R, VEC, begin, end, false),
-            dx(a.dx, b, 0, pl, a.R, VEC, begin, end, false), dg(a.dgate, b, 0, pl, a.R, VEC, begin, end, false);
-        batches<U>(
-            pl.count(a, begin, end),
-            [&](int k) {
-                In i;
-                i.x = V::load(x.at(k));
-                i.g = V::load(g.at(k));
-                i.dy = V::load(d.at(k));
-                return i;
-            },
-            [&](int k, const In& i) {
-                Lanes<VEC> f = V::unpack(i.x), e = V::unpack(i.g), dy = V::unpack(i.dy);
+        Stream<T, VEC, true, true> in(a, b, pl, begin, end, false, smem);
+        in.start();
+        Walk<T> dx(a.dx, b, 0, pl, a.R, VEC, begin, end, false), dg(a.dgate, b, 0, pl, a.R, VEC, begin, end, false);
+        in.run([&](const Input<T, VEC>& i) {
+            Lanes<VEC> f = V::unpack(i.x), e = V::unpack(i.g), dy = V::unpack(i.dy);
 #pragma unroll
-                for (int q = 0; q < Lanes<VEC>::N; ++q)
-                {
-                    float2 value, slope, s, ns;
-                    act_both<T, ACT>(f.p[q], value, slope, a.act);
-                    sigmoid_pair(e.p[q], s, ns);
-                    const float2 ds = mul(dy.p[q], s);
-                    f.p[q] = mul(ds, slope);
-                    e.p[q] = mul(ds, mul(value, ns));
-                }
-                V::store(dx.at(k), f);
-                V::store(dg.at(k), e);
-            },
-            [&](int k) { x.on(k); g.on(k); d.on(k); dx.on(k); dg.on(k); });
+            for (int q = 0; q < Lanes<VEC>::N; ++q)
+            {
+                float2 value, slope, s, ns;
+                act_both<T, ACT>(f.p[q], value, slope, a.act);
+                sigmoid_pair(e.p[q], s, ns);
+                const float2 ds = mul(dy.p[q], s);
+                f.p[q] = mul(ds, slope);
+                e.p[q] = mul(ds, mul(value, ns));
+            }
+            V::store(dx.p, f);
+            V::store(dg.p, e);
+            dx.on(1); dg.on(1);
+        });
     }
 }
 

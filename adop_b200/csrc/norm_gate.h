@@ -66,7 +66,6 @@ struct NormArgs
 // threads of a block and resident blocks of an SM that the kernels are compiled for
 constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
 constexpr int kNormGradThreads = 384, kNormGradBlocks = 2;  // backward
-constexpr int kGateThreads = 512, kGateGradThreads = 256, kGateBlocks = 2;  // the gate alone
 // vectors that the streaming kernels have under way for each thread: a power of two
 __host__ __device__ constexpr int stream_depth(bool gated, bool grad) { return gated ? 4 : 8; }
 constexpr int kParamChannels = 32;  // channels whose parameters' gradients one block adds up

@@ -21,6 +21,7 @@ adop_status refuse(adop_status s, const char* why)
 }
 
 int element_size(int type) { return type == ADOP_TYPE_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 adop_status check_params(const adop_norm_params* p, bool norm)
 {
@@ -39,14 +40,14 @@ adop_status check_params(const adop_norm_params* p, bool norm)
             return refuse(ADOP_ERR_INVALID_ARGUMENT, "num_groups does not divide the channels");
         if (p->param_type != ADOP_TYPE_F32 && p->param_type != p->type)
             return refuse(ADOP_ERR_INVALID_ARGUMENT, "param_type is neither ADOP_TYPE_F32 nor the images' type");
+        const size_t size = p->param_type == ADOP_TYPE_F32 ? 4 : 2;
+        if (!aligned(p->weight, size) || !aligned(p->bias, size)) return refuse(ADOP_ERR_INVALID_ARGUMENT, "weight or bias is not aligned to its type");
         if (!(p->eps >= 0.f) || p->eps > 3.0e38f) return refuse(ADOP_ERR_INVALID_ARGUMENT, "eps is negative or not finite");
     }
     return ADOP_OK;
 }
 
 constexpr int64_t kExtent = (int64_t)1 << 56;  // elements from the first image to the last, and of an image
-
-bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 adop_status check_image(const adop_norm_params* p, const adop_norm_image& im, bool output, const char* what)
 {
@@ -104,10 +105,11 @@ void threads_of(int P, int most, int* R, int* threads)
 // of 33 MB of inputs: 77.8 -> 67.6 us; with the others' launches doubled too, sixteen of them 261 -> 290 us; parts of 35 KB 17.7 -> 19.6 us).
 constexpr int64_t kAlonePart = 64 << 10;  // bytes of one tensor
 
-// Images whose inputs are read twice, by the sums and by what follows, are taken in groups of which the L2 keeps a good part. A group
-// costs two launches (5 us of waits and tails), so two images go together up to the larger bound. Measured: four images of 33 MB of
-// inputs, backward, two by two 78 us, all at once 82 us; sixteen of 50 MB one by one 418 us, two by two 378 us.
-constexpr int64_t kL2Group = 70ll << 20, kL2Pair = 105ll << 20, kGroupCost = 20ll << 20;
+// Images are taken in groups, a launch for the sums and one for what follows each, which costs 5 us of waits and tails a group. Where the
+// second read is bound by memory, forward without a gate, groups that the L2 holds pay (sixteen images of 17 MB, four at a time 135 us,
+// all at once 143 us). With a gate the arithmetic hides the second read (sixteen of 33 MB two at a time 251 us, all at once 230 us). Backward,
+// in between (sixteen of 50 MB two at a time 372 us, four at a time 344 us, all at once 349 us).
+constexpr int64_t kForwardGroup = 70ll << 20, kBackwardGroup = 210ll << 20, kGroupCost = 20ll << 20;
 constexpr int64_t kMinChunk = 16 << 10;  // bytes of one tensor that a block is worth
 
 // How the streaming kernels share out a batch: images of a launch and blocks of an image. By the sizes alone, so that the
@@ -121,8 +123,7 @@ Share share_of(const adop_norm_params* p, bool gated, bool backward)
 {
     const int64_t tensor = p->pixels * p->channels * element_size(p->type);
     const int64_t read = tensor * (1 + (gated ? 1 : 0) + (backward ? 1 : 0));
-    int64_t most = kL2Group / read;
-    if (most < 2 && 2 * read <= kL2Pair) most = 2;
+    int64_t most = backward ? kBackwardGroup / read : gated ? p->batch : kForwardGroup / read;
     if (most > p->batch) most = p->batch;
     if (most < 1) most = 1;
     // groups of one size, the last one too where a few images are a group: its blocks have as much to do as the others'
@@ -319,7 +320,8 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
 {
     ADOP_TRY(check_params(p, true));
     if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
-    if (!io->mean != !io->rstd) return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd are given together or not at all");
+    if (!io->mean != !io->rstd || !aligned(io->mean, 4) || !aligned(io->rstd, 4))
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd are given together or not at all, aligned to their type");
     if (p->batch == 0 || p->pixels == 0) return ADOP_OK;
     const bool gated = io->gate.data != nullptr;
     ADOP_TRY(check_image(p, io->x, false, "x"));
@@ -371,8 +373,8 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
 {
     ADOP_TRY(check_params(p, true));
     if (!io) return refuse(ADOP_ERR_INVALID_ARGUMENT, "no tensors");
-    if ((io->grad_weight && !aligned(io->grad_weight, 2)) || (io->grad_bias && !aligned(io->grad_bias, 2)))
-        return refuse(ADOP_ERR_INVALID_ARGUMENT, "grad_weight or grad_bias");
+    if (!aligned(io->grad_weight, (size_t)element_size(p->param_type)) || !aligned(io->grad_bias, (size_t)element_size(p->param_type)))
+        return refuse(ADOP_ERR_INVALID_ARGUMENT, "grad_weight or grad_bias is not aligned to its type");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (p->batch == 0 || p->pixels == 0)
     {
@@ -382,7 +384,7 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
         return ADOP_OK;
     }
     const bool gated = io->gate.data != nullptr;
-    if (!io->mean || !io->rstd) return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd of the forward call");
+    if (!io->mean || !io->rstd || !aligned(io->mean, 4) || !aligned(io->rstd, 4)) return refuse(ADOP_ERR_INVALID_ARGUMENT, "mean and rstd of the forward call");
     ADOP_TRY(check_image(p, io->x, false, "x"));
     ADOP_TRY(check_image(p, io->grad_y, false, "grad_y"));
     ADOP_TRY(check_image(p, io->grad_x, true, "grad_x"));

@@ -99,6 +99,12 @@ def test_workspace_and_statistics(lib, backward):
     assert call(lib, entry, big, io(workspace=66 * P + 8, **images)) == INVALID
     assert call(lib, entry, params(), io(mean=None)) == INVALID
     assert call(lib, entry, params(), io(rstd=None)) == INVALID
+    assert call(lib, entry, params(), io(mean=64 * P + 2)) == INVALID
+    assert call(lib, entry, params(weight=P + 2), io()) == INVALID
+    assert call(lib, entry, params(bias=P + 1, param_type=capi.TYPE_F16), io()) == INVALID
+    if backward:
+        assert call(lib, entry, params(), io(grad_weight=P + 2)) == INVALID
+        assert call(lib, entry, params(), io(grad_bias=P + 3)) == INVALID
 
 
 @pytest.mark.parametrize("entry", ENTRIES)

@@ -113,8 +113,9 @@ class Reference:
             total = lambda v: v.sum((0, 2, 3))
             pt = max([half_step(p.dtype) for p in (weight, bias) if p is not None], default=0.0)
             self.db, self.dw = total(dz), total(dz * uhat)
-            self.db_tol = pt * self.db.abs() + total(e_dz) + 2.0 ** -21 * total(dz.abs()) + 1e-30
-            self.dw_tol = pt * self.dw.abs() + total(e_dw) + 2.0 ** -21 * total((dz * uhat).abs()) + 1e-30
+            small = max([torch.finfo(p.dtype).smallest_normal * half_step(p.dtype) for p in (weight, bias) if p is not None], default=0.0)
+            self.db_tol = pt * self.db.abs() + total(e_dz) + 2.0 ** -21 * total(dz.abs()) + small
+            self.dw_tol = pt * self.dw.abs() + total(e_dw) + 2.0 ** -21 * total((dz * uhat).abs()) + small
         if g is None:
             self.dx, self.dx_tol = du, h * du.abs() + du_tol + tiny
         else:

@@ -102,13 +102,13 @@ void threads_of(int P, int most, int* R, int* threads)
 }
 
 // The last launch of a backward pass shares the SMs with no other: it gets two blocks an SM where they have something to do (four images
-// of 33 MB of inputs: 77.8 -> 67.6 us; with the others' launches doubled too, sixteen of them 261 -> 290 us; parts of 35 KB 17.7 -> 19.6 us).
+// of 33 MB of inputs 65.1 -> 62.2 us, sixteen 249 -> 232 us, 254 us with the others' launches doubled too; parts of 35 KB 17.7 -> 19.6 us).
 constexpr int64_t kAlonePart = 64 << 10;  // bytes of one tensor
 
 // Images are taken in groups, a launch for the sums and one for what follows each, which costs 5 us of waits and tails a group. Where the
 // second read is bound by memory, forward without a gate, groups that the L2 holds pay (sixteen images of 17 MB, four at a time 135 us,
-// all at once 143 us). With a gate the arithmetic hides the second read (sixteen of 33 MB two at a time 251 us, all at once 230 us). Backward,
-// in between (sixteen of 50 MB two at a time 372 us, four at a time 344 us, all at once 349 us).
+// all at once 141 us). With a gate the arithmetic hides the second read (sixteen of 33 MB two at a time 252 us, all at once 231 us). Backward,
+// in between (sixteen of 50 MB two at a time 372 us, four at a time 346 us, all at once 352 us).
 constexpr int64_t kForwardGroup = 70ll << 20, kBackwardGroup = 210ll << 20, kGroupCost = 20ll << 20;
 constexpr int64_t kMinChunk = 16 << 10;  // bytes of one tensor that a block is worth
 
@@ -136,7 +136,7 @@ Share share_of(const adop_norm_params* p, bool gated, bool backward)
         if (least < 0 || cost < least) { least = cost; images = n; }
     }
     // A block for each SM; backward, the few that add up the parameters' gradients among them: with one more than SMs, two blocks of the
-    // launch that starts early share one (a 1080p frame of 16 channels, backward: 65.6 us, without them 59.0 us).
+    // launch that starts early share one (four 256 x 256 images of 32 channels in fp32, backward: 29.1 us, so 26.3 us).
     const int64_t params = backward && param_blocks_of(p) <= 4 ? param_blocks_of(p) : 0, wave = sm_count() > 8 ? sm_count() - params : sm_count();
     int64_t chunks = wave / images, worth = (tensor + kMinChunk - 1) / kMinChunk;
     if (chunks > worth) chunks = worth;
@@ -154,11 +154,10 @@ size_t sums_scratch(const Shape& sh, int R, int threads) { return sizeof(float) 
 
 // ---- images that stay in a block's shared memory ----------------------------------------------------------------------------
 // A block takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side. One launch in place of two
-// and no workspace: on the host it saves 4 us of 12. On the device a block of 48 KB takes 7 us whatever the others do, two launches over
-// the whole GPU 6 to 8 us; where there is a block for every other SM, 96 KB take as long as two launches do (sixteen images of 1 MB: 13.8
-// against 13.5 us).
+// and no workspace: on the host 6 us in place of 10. On the device a block of 15 KB takes 5.2 us and one of 48 KB 7.0 us, two launches over
+// the whole GPU 5.7 and 5.5 us, so 32 KB; where there is a block for every other SM, 96 KB (sixteen images of 1 MB: 13.7 against 13.6 us).
 constexpr int64_t kSliceBytes = 64;
-constexpr int64_t kResidentBytes = 48 << 10;
+constexpr int64_t kResidentBytes = 32 << 10;
 constexpr int64_t kResidentManyBytes = 96 << 10;
 struct Resident
 {

@@ -18,7 +18,6 @@ enum NormKernel
     kNormKernels
 };
 enum NormVector { kVec16, kVec8, kVec1, kNormVectors };  // bytes of a thread's vector; kVec1 = one element
-constexpr int kNormActs = 5;                             // 0..3 = ADOP_ACTIVATION_*, 4 = chosen at run time
 
 // One channels-last tensor: element (b, pixel, c) at p + b * image + pixel * (row / pixels per row) + c; strides in elements.
 struct NormImage
@@ -63,7 +62,8 @@ struct NormArgs
     float2* channel_part; // [B, chunks, C]
 };
 
-// threads of a block and resident blocks of an SM that the kernels are compiled for
+// Threads of a block and resident blocks of an SM that the kernels are compiled for: 64 registers forward and 80 backward, where a vector's
+// eight channels have four coefficients each. 256 threads with 128 registers hold too few vectors back from memory, 512 with 64 spill.
 constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
 constexpr int kNormGradThreads = 384, kNormGradBlocks = 2;  // backward
 // vectors that the streaming kernels have under way for each thread: a power of two

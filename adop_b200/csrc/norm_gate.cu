@@ -233,8 +233,9 @@ adop_status launch(const Launch& l, const adop_norm_params* p, const Shape& sh, 
     void* args[] = {&a};
     cudaError_t e = cudaSuccess;
     ADOP_LAUNCH(l.name, st, (e = cudaLaunchKernelExC(&cfg, f, args)));
-    if (e != cudaSuccess) return record_cuda_error(e, l.name);
-    return ADOP_OK;
+    if (e == cudaSuccess) return ADOP_OK;
+    cudaGetLastError();  // the caller has it, the next call's checks are not to find it
+    return record_cuda_error(e, l.name);
 }
 
 NormImage image_of(const adop_norm_image& im, const Shape& sh) { return {im.data, im.image_stride, im.pixel_stride * sh.ppr}; }

@@ -595,6 +595,14 @@ static Tensor group_norm_forward(const Tensor& x, const Tensor& weight, const Te
     call_group_norm(adop_group_norm_forward, p, io, false, "adop_group_norm_forward");
     return y;
 }
+// the gradient of an image like `like` with `channels` of them, in channels-last order
+static Tensor upstream_gradient(const Tensor& dy, const Tensor& like, int64_t channels)
+{
+    TORCH_CHECK(dy.device() == like.device() && dy.dim() == 4 && dy.size(0) == like.size(0) && dy.size(1) == channels && dy.size(2) == like.size(2) &&
+                    dy.size(3) == like.size(3),
+                "the gradient has the result's shape and device");
+    return channels_last(dy.scalar_type() == like.scalar_type() ? dy : dy.to(like.scalar_type()));
+}
 static bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
 static void once_differentiable(const char* what)
 {
@@ -623,7 +631,7 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm>
         const bool gated = how % 2 != 0;
         const adop_norm_params p = norm_params(x, weight, bias, stats.size(2), ctx->saved_data["eps"].toDouble(), how / 2, gated);
         c10::cuda::CUDAGuard guard(x.device());
-        Tensor dy = channels_last(grad_output[0]), dx = new_image(x, x.size(1)), dw, db;
+        Tensor dy = upstream_gradient(grad_output[0], x, p.channels), dx = new_image(x, x.size(1)), dw, db;
         adop_norm_io io{};
         io.x = norm_image(x);
         io.grad_y = norm_image(dy);
@@ -689,7 +697,7 @@ struct GatedActivation : public torch::autograd::Function<GatedActivation>
         const Tensor x = ctx->get_saved_variables()[0];
         const adop_norm_params p = norm_params(x, Tensor(), Tensor(), 0, 0.0, ctx->saved_data["activation"].toInt(), true);
         c10::cuda::CUDAGuard guard(x.device());
-        Tensor dy = channels_last(grad_output[0]), dx = new_image(x, x.size(1));
+        Tensor dy = upstream_gradient(grad_output[0], x, p.channels), dx = new_image(x, x.size(1));
         adop_norm_io io{};
         io.x = norm_image(x); io.gate = norm_image(x, p.channels);
         io.grad_y = norm_image(dy);

@@ -368,6 +368,8 @@ def test_upstream_gradients_in_any_order(op):
         assert torch.equal(torch.autograd.grad(y, [x], dy, retain_graph=True)[0], want)
     (s,) = torch.autograd.grad(y.sum(), [x], retain_graph=True)
     assert torch.equal(s, want)
+    for dy in (ones.double(), ones.bfloat16()):  # of another type: as if converted
+        assert torch.equal(torch.autograd.grad(y, [x], dy, retain_graph=True)[0], want)
     # a leaf that is used twice gets both gradients
     two, = torch.autograd.grad(op.group_norm(x, 4, None, None, 1e-5, "silu") + op.group_norm(x, 4, None, None, 1e-5, "silu"), [x], ones)
     assert torch.allclose(two, 2 * want, rtol=1e-6, atol=0)

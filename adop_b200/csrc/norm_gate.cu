@@ -64,7 +64,7 @@ adop_status check_image(const adop_norm_params* p, const adop_norm_image& im, bo
 
 constexpr size_t kMostShared = 220 * 1024;  // of a block
 
-// Vector and row of a call. The widest vector that every tensor's address and strides allow: 16 bytes, 8 bytes or one element.
+// Vector and row of a call. The widest vector that every tensor's address and strides allow: 16, 8 or 4 bytes or one element.
 // A vector either lies within a pixel's channels, or all tensors are dense and a row of lcm(channels, vector) elements holds
 // whole pixels, an even number of times per image.
 struct Shape
@@ -74,9 +74,10 @@ struct Shape
 Shape choose_shape(const adop_norm_params* p, const adop_norm_image* const* images, int n, int from = kVec16)
 {
     const int es = element_size(p->type);
-    for (int vec = from; vec <= kVec8; ++vec)
+    for (int vec = from; vec < kVec1; ++vec)
     {
-        const int V = (vec == kVec16 ? 16 : 8) / es;
+        const int V = (16 >> vec) / es;
+        if (V < 2) break;
         bool ok = true, dense = true;
         for (int i = 0; i < n; ++i)
         {
@@ -147,6 +148,7 @@ constexpr size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 size_t group_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->num_groups); }
 size_t channel_part_bytes(const adop_norm_params* p, int chunks) { return align16(sizeof(float2) * p->batch * (size_t)chunks * p->channels); }
 
+constexpr size_t kWarpScratch = sizeof(double2) * (kNormThreads / 32);  // group_sums'
 // the block's sums, as the kernels lay them out: block_moments' with the counts, block_sums'
 size_t sum_rows(const Shape& sh, int R, int threads) { return (size_t)(32 % sh.P == 0 ? threads / 32 : R) * sh.P; }
 size_t moments_scratch(const Shape& sh, int m, int R, int threads) { return sizeof(float) * (2 * (sh.V / m) + 1) * sum_rows(sh, R, threads); }
@@ -184,7 +186,7 @@ bool resident_of(const adop_norm_params* p, const Shape& sh, bool gated, Residen
         const bool many = ((int64_t)p->batch << log2) * 2 >= sm_count();
         if (vectors > (many ? kResidentManyBytes : kResidentBytes)) continue;
         const int m = (int)gcd64(p->channels / p->num_groups, sh.V);
-        c.fixed = align16(sizeof(float2) * G + sizeof(float) * 2 * (size_t)C + moments_scratch(s, m, c.R, c.threads));
+        c.fixed = align16(kWarpScratch + sizeof(float2) * G + sizeof(float) * 2 * (size_t)C + moments_scratch(s, m, c.R, c.threads));
         c.smem = c.fixed + (size_t)vectors;
         if (c.smem > kMostShared) continue;
         *r = c;
@@ -270,7 +272,10 @@ void finish(NormArgs* a, int threads, int chunks)
     };
     const int rows = 32 % a->P == 0 ? threads / 32 : a->R;
     a->row_lanes = log2_of(rows);
-    a->lanes = log2_of((int64_t)(1 << a->row_lanes) * (a->Cg / a->m * a->ppr));
+    const int slots = a->Cg / a->m * a->ppr;
+    a->lanes = log2_of((int64_t)(1 << a->row_lanes) * slots);
+    // few groups of many sums: more warps than one each
+    a->warps = rows * slots > 64 && a->G * 2 <= threads / 32 ? threads / 32 / a->G : 1;
         a->sums = a->own = parts_of(a->rows, chunks);
     const double per_row = (double)a->ppr * a->Cg;
     a->inv_n = 1.0 / (a->rows * per_row);
@@ -351,7 +356,7 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     threads_of(a.P, kNormThreads, &a.R, &threads);
     const Share share = share_of(p, gated, false);
     finish(&a, threads, share.chunks < a.rows ? share.chunks : a.rows);
-    const size_t smem_stats = moments_scratch(sh, a.m, a.R, threads);
+    const size_t smem_stats = kWarpScratch + moments_scratch(sh, a.m, a.R, threads);
     const size_t smem_apply = apply_smem(a);
     const int es = element_size(p->type);
     for (a.image0 = 0; a.image0 < p->batch; a.image0 += share.images)

@@ -530,18 +530,21 @@ __device__ __forceinline__ void block_moments(Lanes<VEC> (&v)[2], const Lanes<VE
     put_moments_of<VEC, 1>(v, pivot, n, a, pl, buf, counts);
 }
 
-// The block's sums of u and u^2 of a group in 64 bits, for f(g, sums), from what block_moments left.
-template <int VEC, class F> __device__ __forceinline__ void group_sums(const NormArgs& a, const float* buf, const float* counts, F f)
+// The block's sums of u and u^2 of a group in 64 bits, for f(g, sums), from what block_moments left: by 2^a.lanes threads a group, or by
+// a.warps whole warps, which meet in scratch of a double2 each. Barriers where it takes some.
+template <int VEC, class F> __device__ __forceinline__ void group_sums(const NormArgs& a, const float* buf, const float* counts, double2* scratch, F f)
 {
     const int sh = __ffs(a.m) - 1, per = VEC >> sh, run = a.Cg >> sh, slots = run * a.ppr, rows = sum_rows(a), second = per * rows * a.P;
-    const int lanes = 1 << a.lanes, row_lanes = 1 << a.row_lanes, want = ((a.G << a.lanes) + 31) & ~31;
+    const int lanes = 1 << a.lanes, row_lanes = 1 << a.row_lanes, want = ((a.G << a.lanes) * a.warps + 31) & ~31;
     for (int idx = threadIdx.x; idx < want; idx += blockDim.x)
     {
         // a group's lanes: row_lanes for a slot's rows, so many slots at a time
-        const int g = idx >> a.lanes, lane = idx & (lanes - 1), row = lane & (row_lanes - 1);
+        int g = idx >> a.lanes, part = 0;
+        const int lane = idx & (lanes - 1), row = lane & (row_lanes - 1);
+        if (a.warps > 1) { part = g % a.warps; g /= a.warps; }
         double s = 0.0, q = 0.0;
         if (g < a.G)
-            for (int slot = lane >> a.row_lanes; slot < slots; slot += lanes >> a.row_lanes)
+            for (int slot = (part << (a.lanes - a.row_lanes)) + (lane >> a.row_lanes); slot < slots; slot += (lanes >> a.row_lanes) * a.warps)
             {
                 int i = slot, e = g * a.Cg;
                 while (i >= run) { i -= run; e += a.C; }
@@ -560,7 +563,19 @@ template <int VEC, class F> __device__ __forceinline__ void group_sums(const Nor
             s += __shfl_xor_sync(0xffffffffu, s, o);
             q += __shfl_xor_sync(0xffffffffu, q, o);
         }
-        if (g < a.G && lane == 0) f(g, make_double2(s, q));
+        if (g < a.G && lane == 0)
+        {
+            if (a.warps == 1) f(g, make_double2(s, q));
+            else scratch[g * a.warps + part] = make_double2(s, q);
+        }
+    }
+    if (a.warps == 1) return;
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.G; g += blockDim.x)
+    {
+        double2 sum = scratch[g * a.warps];
+        for (int k = 1; k < a.warps; ++k) { sum.x += scratch[g * a.warps + k].x; sum.y += scratch[g * a.warps + k].y; }
+        f(g, sum);
     }
 }
 
@@ -654,7 +669,7 @@ template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>&
 // (132 MB from and to the L2). Sums of gated values, where the arithmetic counts: 4.4 TB/s over 537 MB; results 5.7 to 6.1 TB/s.
 // Tried and slower: one launch whose blocks take tiles of both kinds by a counter (four images of 33 MB of inputs, backward 97 us against
 // 78 us then), clusters that keep an image in their shared memory (sixteen of 1 MB 16.2 us against 13.5 us).
-// Shared memory: block_moments' scratch | vectors
+// Shared memory: double2 scratch[16] | block_moments' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const __grid_constant__ NormArgs a)
 {
@@ -663,7 +678,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
     const int b = a.image0 + blockIdx.y;
     int begin, end;
     chunk_of(a, blockIdx.x, begin, end);
-    float* buf = reinterpret_cast<float*>(smem);
+    double2* scratch = smem;
+    float* buf = reinterpret_cast<float*>(smem + kNormThreads / 32);
     float* counts = buf + 2 * (VEC / a.m) * sum_rows(a) * a.P;
     for (int ph0 = 0; ph0 < a.P; ph0 += blockDim.x)
     {
@@ -684,7 +700,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
     __syncthreads();
     float2* out = a.group_part + (size_t)b * a.sums.count * a.G + blockIdx.x;
     const double inv_n = (int)blockIdx.x < a.sums.more ? a.inv_long : a.inv_short;
-    group_sums<VEC>(a, buf, counts, [&](int g, double2 sums) {
+    group_sums<VEC>(a, buf, counts, scratch, [&](int g, double2 sums) {
         // the chunk's mean and sum of squares about it: 32 bits hold these
         const double mean = sums.x * inv_n;
         out[(size_t)g * a.sums.count] = make_float2((float)mean, (float)fma(-mean, sums.x, sums.y));
@@ -830,9 +846,24 @@ __device__ __forceinline__ void input_gradient(const Input<T, VEC>& in, const Ba
 }
 // channel sums chan[2][C] from the slots' (a row may hold several pixels), then f(g, the group's sums of w dz and w dz uhat)
 template <int VEC, class F>
-__device__ __forceinline__ void channel_and_group_sums(const NormArgs& a, const float* params, const float* buf, float* chan, F f)
+__device__ __forceinline__ void channel_and_group_sums(const NormArgs& a, const float* params, float* buf, float* chan, F f)
 {
-    const int T = blockDim.x, t = threadIdx.x, rows = sum_rows(a);
+    const int T = blockDim.x, t = threadIdx.x;
+    int rows = sum_rows(a);
+    // many rows of few columns: all threads take some first
+    const int columns = 2 * VEC * a.P, parts = T / columns;
+    if (parts > 1 && rows > 2 * parts)
+    {
+        const int part = t / columns, i = t - part * columns, slot = i / a.P;
+        float s = 0.f;
+        if (part < parts)
+#pragma unroll 4
+            for (int r = part; r < rows; r += parts) s += buf[(slot * rows + r) * a.P + i - slot * a.P];
+        __syncthreads();
+        if (part < parts) buf[(slot * parts + part) * a.P + i - slot * a.P] = s;
+        __syncthreads();
+        rows = parts;
+    }
     for (int i = t; i < 2 * a.C; i += T)
     {
         const int k = i >= a.C, c = i - k * a.C;
@@ -1018,13 +1049,14 @@ template <class Copy, class Between, class Use> __device__ __forceinline__ void 
     for (int i = 3 * quarter; i < n; ++i) use(i);
 }
 
-// Shared memory: float2 stat[G] | float params[2 C] | block_moments' scratch | vectors
+// Shared memory: double2 scratch[16] | float2 stat[G] | float params[2 C] | block_moments' scratch | vectors
 template <typename T, int VEC, bool GATED, int ACT>
 __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(const __grid_constant__ NormArgs a)
 {
     extern __shared__ double2 smem[];
     const int T_ = blockDim.x, b = blockIdx.x >> a.slices, slice = blockIdx.x - (b << a.slices), c0 = slice * a.C;
-    float2* stat = reinterpret_cast<float2*>(smem);
+    double2* scratch = smem;
+    float2* stat = reinterpret_cast<float2*>(smem + kNormThreads / 32);
     float* params = reinterpret_cast<float*>(stat + a.G);
     float* buf = params + 2 * a.C;
     float* counts = buf + 2 * (VEC / a.m) * sum_rows(a) * a.P;
@@ -1036,7 +1068,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
     W* sg = sx + (size_t)most * T_;
     const Place pl(a, 0);
     const int n = pl.active ? pl.count(a, 0, a.rows) : 0;
-    constexpr int H = Lanes<VEC>::N / 2;  // u in 32 bits takes the room of x and of the gate, or of x alone
+    // u in 32 bits takes the room of x and of the gate, or of x alone
     Lanes<VEC> v[2], pivot;
     v[0].fill(0.f); v[1].fill(0.f); pivot.fill(0.f);
     Walk<T> x(a.x, b, c0, pl, a.R, VEC, 0, a.rows, false), g(a.gate, b, c0, pl, a.R, VEC, 0, a.rows, false);
@@ -1063,18 +1095,14 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
             add_moments<VEC>(u, pivot, v);
             if constexpr (GATED)
             {
-                if constexpr (sizeof(T) == 4) sx[i * T_] = *reinterpret_cast<const W*>(&u);
-                else
-                {
-                    sx[i * T_] = *reinterpret_cast<const W*>(&u.p[0]);
-                    sg[i * T_] = *reinterpret_cast<const W*>(&u.p[H]);
-                }
+                sx[i * T_] = *reinterpret_cast<const W*>(&u);
+                if constexpr (sizeof(T) == 2) sg[i * T_] = *reinterpret_cast<const W*>(reinterpret_cast<const char*>(&u) + V::kBytes);
             }
         });
     block_moments<VEC>(v, pivot, n, a, pl, buf, counts);
     __syncthreads();
     const size_t g0 = (size_t)blockIdx.x * a.G;
-    group_sums<VEC>(a, buf, counts, [&](int i, double2 sums) {
+    group_sums<VEC>(a, buf, counts, scratch, [&](int i, double2 sums) {
         const float2 s = mean_rstd(sums, a.inv_n, a.eps);
         stat[i] = s;
         if (a.mean)
@@ -1094,11 +1122,10 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_resident(con
         Lanes<VEC> u;
         const W w = sx[i * T_];
         if constexpr (!GATED) u = V::unpack(w);
-        else if constexpr (sizeof(T) == 4) *reinterpret_cast<W*>(&u) = w;
         else
         {
-            *reinterpret_cast<W*>(&u.p[0]) = w;
-            *reinterpret_cast<W*>(&u.p[H]) = sg[i * T_];
+            *reinterpret_cast<W*>(&u) = w;
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<W*>(reinterpret_cast<char*>(&u) + V::kBytes) = sg[i * T_];
         }
         normalise<T, VEC, GATED, ACT>(u, f, a.act);
         V::store(y.p, u);
@@ -1196,6 +1223,8 @@ template <typename T> const void* norm_kernel(int which, int vec, bool gated, in
     constexpr int V16 = 16 / sizeof(T), V8 = 8 / sizeof(T);
     if (vec == kVec16) return gated ? pick_act<T, V16, true>(which, act) : pick_act<T, V16, false>(which, act);
     if (vec == kVec8) return gated ? pick_act<T, V8, true>(which, act) : pick_act<T, V8, false>(which, act);
+    if constexpr (sizeof(T) == 2)
+        if (vec == kVec4) return gated ? pick<T, 2, true, 4>(which) : pick<T, 2, false, 4>(which);
     return gated ? pick_act<T, 1, true>(which, act) : pick_act<T, 1, false>(which, act);
 }
 

@@ -17,7 +17,7 @@ enum NormKernel
     kGateGrad,          // df, dg
     kNormKernels
 };
-enum NormVector { kVec16, kVec8, kVec1, kNormVectors };  // bytes of a thread's vector; kVec1 = one element
+enum NormVector { kVec16, kVec8, kVec4, kVec1, kNormVectors };  // bytes of a thread's vector; kVec1 = one element (kVec4: of 16-bit images)
 
 // One channels-last tensor: element (b, pixel, c) at p + b * image + pixel * (row / pixels per row) + c; strides in elements.
 struct NormImage
@@ -41,7 +41,8 @@ struct NormArgs
     int P, ppr;       // vectors and pixels of a row
     int R;            // rows that a block takes at once (1 when a row has more vectors than the block threads)
     int m;            // channels of a thread's vector that share a group: gcd(Cg, VEC)
-    int lanes, row_lanes;  // log2 of the threads that add up one group's sums, and of those for one slot's rows
+    int lanes, row_lanes;  // log2 of the threads of a warp that add up one group's sums, and of those for one slot's rows
+    int warps;        // warps that add up one group's sums
     int rows;         // rows of an image
     int image0;       // first image of the launch
     NormParts sums;   // parts of an image that have a partial sum each

@@ -123,6 +123,23 @@ __device__ __forceinline__ float load_param(const void* p, int type, int i)
     if (type == ADOP_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
+// f(i, load(i)) for i = first, first + step, ... below end: four loads are under way before the first is used. An unrolled loop takes its
+// remainder one load after the other, and the two or three partial sums of a thread are all remainder: an image of 320 x 180 x 32 in bfloat16
+// takes 7.9 us forward for 8.8 and 10.4 backward for 11.6. Eight loads cost k_norm_grad_apply its registers: 270 us backward for 226 of 16 images
+// of 960 x 540 x 16.
+template <class Load, class F> __device__ __forceinline__ void four_at_a_time(int first, int step, int end, Load load, F f)
+{
+    for (int i = first; i < end; i += 4 * step)
+    {
+        decltype(load(0)) v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * step < end) v[k] = load(i + k * step);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * step < end) f(i + k * step, v[k]);
+    }
+}
 // weight and bias of the channels from c0 on as to[C] and to[C] behind it, 1 and 0 where there are none; a barrier follows
 __device__ __forceinline__ void stage_params(const NormArgs& a, int c0, float* to)
 {
@@ -591,12 +608,12 @@ __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part par
         const int g = idx >> a.gather, lane = idx & (lanes - 1);
         double2 sum = make_double2(0.0, 0.0);
         if (g < a.G)
-#pragma unroll 8
-            for (int k = lane; k < a.sums.count; k += lanes)
-            {
-                const double2 v = part(k, __ldcg(from + (size_t)g * a.sums.count + k));
-                sum.x += v.x; sum.y += v.y;
-            }
+            four_at_a_time(
+                lane, lanes, a.sums.count, [&](int k) { return __ldcg(from + (size_t)g * a.sums.count + k); },
+                [&](int k, float2 of) {
+                    const double2 v = part(k, of);
+                    sum.x += v.x; sum.y += v.y;
+                });
         for (int o = lanes >> 1; o > 0; o >>= 1)
         {
             sum.x += __shfl_xor_sync(0xffffffffu, sum.x, o);
@@ -917,13 +934,14 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
     {
         const Place pl(a, ph0);
         Stream<T, VEC, GATED, true> in(a, b, pl, begin, end, false, smem);
-        in.start();
         if (ph0 == 0)
         {
+            // before the copies, behind which they would wait 5 us for their values
             stage_params(a, 0, params);
             stage_stats(a, (size_t)b * a.G, stat);
-            __syncthreads();
         }
+        in.start();
+        if (ph0 == 0) __syncthreads();
         Lanes<VEC> v[2];
         v[0].fill(0.f); v[1].fill(0.f);
         if (pl.active)
@@ -951,12 +969,9 @@ __device__ __forceinline__ void param_gradients(const NormArgs& a, int c0, int n
     const int w = t / nc, c = t - w * nc;
     double s = 0.0, q = 0.0;
     if (w < ways)
-#pragma unroll 8
-        for (int k = w; k < a.param_parts; k += ways)
-        {
-            const float2 v = __ldcg(a.channel_part + (size_t)k * a.C + c0 + c);
-            s += v.x; q += v.y;
-        }
+        four_at_a_time(
+            w, ways, a.param_parts, [&](int k) { return __ldcg(a.channel_part + (size_t)k * a.C + c0 + c); },
+            [&](int, float2 v) { s += v.x; q += v.y; });
     scratch[2 * t] = s;
     scratch[2 * t + 1] = q;
     __syncthreads();

@@ -156,8 +156,9 @@ size_t sums_scratch(const Shape& sh, int R, int threads) { return sizeof(float) 
 
 // ---- images that stay in a block's shared memory ----------------------------------------------------------------------------
 // A block takes one of 2^slices channel ranges of an image, whole groups of at least kSliceBytes side by side. One launch in place of two
-// and no workspace: on the host 6 us in place of 10. On the device a block of 15 KB takes 5.2 us and one of 48 KB 7.0 us, two launches over
-// the whole GPU 5.7 and 5.5 us, so 32 KB; where there is a block for every other SM, 96 KB (sixteen images of 1 MB: 13.7 against 13.6 us).
+// and no workspace: on the host 6 us in place of 10. On the device a block of 15 KB takes 5.1 us and one of 32 KB 6.2 us, two launches over
+// the whole GPU 5.4 and 5.8 us, so 32 KB; where there is a block for every other SM, 96 KB (256 images of 16 KB: 7.4 against 8.7 us, sixteen
+// of 1 MB 13.6 against 13.8 us).
 constexpr int64_t kSliceBytes = 64;
 constexpr int64_t kResidentBytes = 32 << 10;
 constexpr int64_t kResidentManyBytes = 96 << 10;

@@ -123,20 +123,19 @@ __device__ __forceinline__ float load_param(const void* p, int type, int i)
     if (type == ADOP_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
-// f(i, load(i)) for i = first, first + step, ... below end: four loads are under way before the first is used. An unrolled loop takes its
+// f(i, load(i)) for i = first, first + step, ... below end: N loads are under way before the first is used. An unrolled loop takes its
 // remainder one load after the other, and the two or three partial sums of a thread are all remainder: an image of 320 x 180 x 32 in bfloat16
-// takes 7.9 us forward for 8.8 and 10.4 backward for 11.6. Eight loads cost k_norm_grad_apply its registers: 270 us backward for 226 of 16 images
-// of 960 x 540 x 16.
-template <class Load, class F> __device__ __forceinline__ void four_at_a_time(int first, int step, int end, Load load, F f)
+// takes 7.9 us forward for 8.8 and 10.4 backward for 11.6.
+template <int N, class Load, class F> __device__ __forceinline__ void loads_ahead(int first, int step, int end, Load load, F f)
 {
-    for (int i = first; i < end; i += 4 * step)
+    for (int i = first; i < end; i += N * step)
     {
-        decltype(load(0)) v[4];
+        decltype(load(0)) v[N];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < N; ++k)
             if (i + k * step < end) v[k] = load(i + k * step);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < N; ++k)
             if (i + k * step < end) f(i + k * step, v[k]);
     }
 }
@@ -597,8 +596,10 @@ template <int VEC, class F> __device__ __forceinline__ void group_sums(const Nor
 }
 
 // f(g, sums) for the groups of an image from the partial sums [G, chunks] of its chunks, part(k, v) = what partial sum k stands for in
-// 64 bits; by 2^a.gather threads a group. The caller waits at a barrier.
-template <class Part, class F>
+// 64 bits; by 2^a.gather threads a group. The caller waits at a barrier. AHEAD partial sums of a thread are loaded at once: four, but two in
+// the gated backward pass, whose loop is short of registers (16 images of 960 x 540 x 16 in bfloat16: 345 us with two, 354 with four; eight
+// 402, and 270 for 226 without a gate).
+template <int AHEAD, class Part, class F>
 __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part part, F f)
 {
     const float2* __restrict__ from = a.group_part + (size_t)b * a.sums.count * a.G;
@@ -608,7 +609,7 @@ __device__ __forceinline__ void gather_groups(const NormArgs& a, int b, Part par
         const int g = idx >> a.gather, lane = idx & (lanes - 1);
         double2 sum = make_double2(0.0, 0.0);
         if (g < a.G)
-            four_at_a_time(
+            loads_ahead<AHEAD>(
                 lane, lanes, a.sums.count, [&](int k) { return __ldcg(from + (size_t)g * a.sums.count + k); },
                 [&](int k, float2 of) {
                     const double2 v = part(k, of);
@@ -681,8 +682,8 @@ template <int VEC> __device__ __forceinline__ void add_moments(const Lanes<VEC>&
 // Two launches, sums and what follows, a block on each SM for either. Both take less than half an SM and may start while the launch in
 // front of them runs: the next images' sums and these images' results share the SMs, and a launch has its first vectors when its turn
 // comes. Between blocks only the partial sums pass, so nobody waits for a block that may not be resident.
-// A 1080p frame of 16 channels in 16 bits (66 MB in, 66 MB out) takes 34.5 us: the sums 14 us (66 MB from HBM beside what the L2 writes back
-// of the call before; 10.5 us on a clean L2, 6.3 TB/s), 2 us to the partial sums, 1 us of wait, 2 us to mean and rstd, the results 11 us
+// A 1080p frame of 16 channels in 16 bits (66 MB in, 66 MB out) takes 33.5 us: the sums 14 us (66 MB from HBM beside what the L2 writes back
+// of the call before; 10.5 us on a clean L2, 6.3 TB/s), 2 us to the partial sums, 1 us of wait, 1 us to mean and rstd, the results 11 us
 // (132 MB from and to the L2). Sums of gated values, where the arithmetic counts: 4.4 TB/s over 537 MB; results 5.7 to 6.1 TB/s.
 // Tried and slower: one launch whose blocks take tiles of both kinds by a counter (four images of 33 MB of inputs, backward 97 us against
 // 78 us then), clusters that keep an image in their shared memory (sixteen of 1 MB 16.2 us against 13.5 us).
@@ -747,7 +748,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_apply(const 
             stage_params(a, 0, params);
             wait_previous();
             const double per_row = (double)(a.ppr * a.Cg);
-            gather_groups(
+            gather_groups<4>(
                 a, b,
                 [&](int k, float2 v) {
                     const double mean = v.x, s = (double)(a.sums.rows + (k < a.sums.more ? 1 : 0)) * per_row * mean;
@@ -969,7 +970,7 @@ __device__ __forceinline__ void param_gradients(const NormArgs& a, int c0, int n
     const int w = t / nc, c = t - w * nc;
     double s = 0.0, q = 0.0;
     if (w < ways)
-        four_at_a_time(
+        loads_ahead<4>(
             w, ways, a.param_parts, [&](int k) { return __ldcg(a.channel_part + (size_t)k * a.C + c0 + c); },
             [&](int, float2 v) { s += v.x; q += v.y; });
     scratch[2 * t] = s;
@@ -1016,7 +1017,7 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
             stage_params(a, 0, params);
             stage_stats(a, (size_t)b * a.G, stat);
             wait_previous();
-            gather_groups(
+            gather_groups<GATED ? 2 : 4>(
                 a, b, [&](int, float2 v) { return make_double2(v.x, v.y); },
                 [&](int g, double2 sums) { c12[g] = make_float2((float)(sums.x * a.inv_n), (float)(sums.y * a.inv_n)); });
             __syncthreads();
@@ -1042,7 +1043,7 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
 // ---- images that fit a block's shared memory ----------------------------------------------------------------------------------
 // A block keeps an image, or some groups' channels of it, between the sums and what follows: one launch, every value read once. A
 // thread copies, reads and overwrites vectors of its own only. Bound by the latency of the one chain from the first copy to the last store:
-// 5.2 us for 120 pixels of 64 channels.
+// 5.1 us for 120 pixels of 64 channels.
 // n vectors in four groups: all copies are under way before the first group is used
 template <class Copy, class Between, class Use> __device__ __forceinline__ void staged(int n, int most, Copy copy, Between between, Use use)
 {

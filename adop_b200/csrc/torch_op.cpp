@@ -604,9 +604,16 @@ static Tensor upstream_gradient(const Tensor& dy, const Tensor& like, int64_t ch
     return channels_last(dy.scalar_type() == like.scalar_type() ? dy : dy.to(like.scalar_type()));
 }
 static bool wants_gradient(const Tensor& t) { return t.defined() && t.requires_grad(); }
-static void once_differentiable(const char* what)
+// A tangent (forward-mode differentiation) is carried by a tensor whose requires_grad is false, with gradients enabled or not: a call that
+// wrote its result beside it would answer with a derivative of zero.
+template <class... Tensors> static void no_tangent(const char* what, const Tensors&... t)
+{
+    TORCH_CHECK(!((t.defined() && t._fw_grad(0).defined()) || ...), what, " has no forward-mode derivative: its inputs and their gradients carry no tangents (make_dual, jvp)");
+}
+static void once_differentiable(const char* what, const Tensor& dy)
 {
     TORCH_CHECK(!torch::GradMode::is_enabled(), what, " has no second derivative: its gradients cannot be recorded (create_graph)");
+    no_tangent(what, dy);
 }
 
 struct GroupNorm : public torch::autograd::Function<GroupNorm>
@@ -624,7 +631,7 @@ struct GroupNorm : public torch::autograd::Function<GroupNorm>
     }
     static variable_list backward(AutogradContext* ctx, variable_list grad_output)
     {
-        once_differentiable("group_norm");
+        once_differentiable("group_norm", grad_output[0]);
         auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
         const int64_t how = ctx->saved_data["how"].toInt();
@@ -655,7 +662,9 @@ static Tensor group_norm_call(const Tensor& x, int64_t groups, const c10::option
     TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
     TORCH_CHECK(groups > 0, "num_groups is positive");
     const int64_t act = activation_of(activation);
-    const Tensor xc = channels_last(x), w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
+    const Tensor w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
+    no_tangent("group_norm", x, w, b);
+    const Tensor xc = channels_last(x);
     if (torch::GradMode::is_enabled() && (wants_gradient(x) || wants_gradient(w) || wants_gradient(b)))
         return GroupNorm::apply(xc, weight, bias, groups, eps, act, gated);
     return group_norm_forward(xc, w, b, groups, eps, act, gated, Tensor());
@@ -693,7 +702,7 @@ struct GatedActivation : public torch::autograd::Function<GatedActivation>
     }
     static variable_list backward(AutogradContext* ctx, variable_list grad_output)
     {
-        once_differentiable("gated_activation");
+        once_differentiable("gated_activation", grad_output[0]);
         const Tensor x = ctx->get_saved_variables()[0];
         const adop_norm_params p = norm_params(x, Tensor(), Tensor(), 0, 0.0, ctx->saved_data["activation"].toInt(), true);
         c10::cuda::CUDAGuard guard(x.device());
@@ -710,6 +719,7 @@ static Tensor gated_activation(const Tensor& x, std::string activation)
 {
     TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,2C,H,W]");
     const int64_t act = activation_of(activation);
+    no_tangent("gated_activation", x);
     const Tensor xc = channels_last(x);
     if (torch::GradMode::is_enabled() && wants_gradient(x)) return GatedActivation::apply(xc, act);
     return gated_forward(xc, act);

@@ -518,10 +518,12 @@ static bool pixel_stride(const Tensor& t, int64_t* stride)
     *stride = W > 1 ? t.stride(3) : (H > 1 ? t.stride(2) : C);
     return (C == 1 || t.stride(1) == 1) && (H <= 1 || W <= 1 || t.stride(2) == W * t.stride(3));
 }
+// A view that stands for the negative of what its memory holds (the imaginary part of a conjugate, and the gradient of one) is written out.
+static Tensor as_stored(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 static Tensor channels_last(const Tensor& t)
 {
     int64_t stride;
-    return t.numel() == 0 || pixel_stride(t, &stride) ? t : t.contiguous(torch::MemoryFormat::ChannelsLast);
+    return as_stored(t.numel() == 0 || pixel_stride(t, &stride) ? t : t.contiguous(torch::MemoryFormat::ChannelsLast));
 }
 // channels [c0, ...) of t
 static adop_norm_image norm_image(const Tensor& t, int64_t c0 = 0)
@@ -662,11 +664,11 @@ static Tensor group_norm_call(const Tensor& x, int64_t groups, const c10::option
     TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
     TORCH_CHECK(groups > 0, "num_groups is positive");
     const int64_t act = activation_of(activation);
-    const Tensor w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
+    const Tensor w = as_stored(weight ? *weight : Tensor()), b = as_stored(bias ? *bias : Tensor());
     no_tangent("group_norm", x, w, b);
     const Tensor xc = channels_last(x);
     if (torch::GradMode::is_enabled() && (wants_gradient(x) || wants_gradient(w) || wants_gradient(b)))
-        return GroupNorm::apply(xc, weight, bias, groups, eps, act, gated);
+        return GroupNorm::apply(xc, weight ? c10::make_optional(w) : weight, bias ? c10::make_optional(b) : bias, groups, eps, act, gated);
     return group_norm_forward(xc, w, b, groups, eps, act, gated, Tensor());
 }
 static Tensor group_norm(const Tensor& x, int64_t num_groups, const c10::optional<Tensor>& weight, const c10::optional<Tensor>& bias, double eps,

@@ -47,3 +47,47 @@ def test_functional_jvp_is_refused(op):
     for kind in ("norm", "gate", "gated_norm"):
         with pytest.raises(RuntimeError):
             torch.func.jvp(lambda v: call(op, kind, v, 2, None, None, 1e-5, "elu"), (x,), (torch.ones_like(x),))
+
+
+# ---- tensors whose values are not as stored ---------------------------------------------------------------------------------------
+def negated(t):
+    """t's values as a view of their negatives."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+@pytest.mark.parametrize("kind", ["norm", "gate", "gated_norm"])
+def test_negated_views_are_taken_for_their_values(op, kind):
+    gen = generator(4)
+    C = 8 if kind == "norm" else 16
+    x, dy = image((2, C, 6, 7), torch.float32, gen), image((2, 8, 6, 7), torch.float32, gen)
+    w, b = torch.randn(8, device=DEV, generator=gen), torch.randn(8, device=DEV, generator=gen)
+    want = call(op, kind, x, 2, w, b, 1e-5, "elu")
+    assert torch.equal(call(op, kind, negated(x), 2, negated(w), negated(b), 1e-5, "elu"), want)
+    leaves = [t.clone(memory_format=torch.preserve_format).requires_grad_(True) for t in ((x,) if kind == "gate" else (x, w, b))]
+    through = lambda f: call(op, kind, f(leaves[0]), 2, *(f(t) for t in leaves[1:]), 1e-5, "elu") if kind != "gate" else call(op, kind, f(leaves[0]), 0, None, None, 0, "elu")
+    plain = torch.autograd.grad(through(lambda t: t), leaves, dy)
+    y = through(lambda t: torch._neg_view(t.neg()))
+    assert torch.equal(y, want)
+    for got, grad in zip(torch.autograd.grad(y, leaves, negated(dy)), plain):
+        assert torch.equal(got, grad)
+
+
+def test_the_gradient_of_an_imaginary_part(op):
+    """The upstream gradient is a view of a conjugate there: one channel, pixels two elements apart, negated."""
+    gen = generator(5)
+    x = image((2, 2, 6, 7), torch.float32, gen).requires_grad_(True)
+    re, scale = (torch.randn((2, 1, 6, 7), device=DEV, generator=gen) for _ in range(2))
+    seen = []
+    y = op.gated_activation(x)
+    y.register_hook(lambda g: seen.append(g.is_neg()))
+    # |re + i y|^2 / 2 by way of a conjugate: dy = y scale
+    loss = (torch.complex(re, y).conj().resolve_conj().abs().square() * scale).sum() / 2
+    got, = torch.autograd.grad(loss, [x])
+    assert seen == [True]
+    want, = torch.autograd.grad(op.gated_activation(x), [x], y.detach() * scale)
+    # dy by way of abs(): some rounding steps of 2^-24 of |re|^2 + y^2 over |z|; gx is dy times factors of at most 1.1
+    bound = 2.0 ** -20 * (re.abs() + y.detach().abs()) * scale.abs() * 1.1 * (1 + x.detach().abs().sum(1, keepdim=True))
+    assert bool(((got - want).abs() <= bound).all())
+    assert bool((want.abs() > 4 * bound).any())

@@ -662,7 +662,8 @@ static Tensor group_norm_call(const Tensor& x, int64_t groups, const c10::option
                               const std::string& activation, bool gated)
 {
     TORCH_CHECK(x.is_cuda() && x.dim() == 4, "x: CUDA [B,C,H,W]");
-    TORCH_CHECK(groups > 0, "num_groups is positive");
+    // before the statistics' tensor, which is as large as num_groups says
+    TORCH_CHECK(groups > 0 && groups <= x.size(1), "num_groups is positive and divides the channels, not ", groups);
     const int64_t act = activation_of(activation);
     const Tensor w = as_stored(weight ? *weight : Tensor()), b = as_stored(bias ? *bias : Tensor());
     no_tangent("group_norm", x, w, b);

@@ -91,3 +91,16 @@ def test_the_gradient_of_an_imaginary_part(op):
     bound = 2.0 ** -20 * (re.abs() + y.detach().abs()) * scale.abs() * 1.1 * (1 + x.detach().abs().sum(1, keepdim=True))
     assert bool(((got - want).abs() <= bound).all())
     assert bool((want.abs() > 4 * bound).any())
+
+
+# ---- refusals of a recorded call ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("groups", [0, -4, 5, 17, 1 << 20, (1 << 31) - 1, 1 << 40, (1 << 63) - 1])
+def test_groups_are_checked_before_anything_is_allocated_for_them(op, groups):
+    x = image((2, 16, 6, 7), torch.float32, generator(6)).requires_grad_(True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for kind in ("norm", "gated_norm"):
+        with pytest.raises(RuntimeError, match="num_groups"):
+            call(op, kind, x, groups, None, None, 1e-5, "elu")
+    assert torch.cuda.max_memory_allocated() <= before + (1 << 20)

@@ -693,9 +693,9 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
 {
     extern __shared__ double2 smem[];
     let_next_start();
-    const int b = a.image0 + blockIdx.y;
+    const int b = a.image0 + blockIdx.y, part = a.part0 + blockIdx.x * a.part_step;
     int begin, end;
-    chunk_of(a, blockIdx.x, begin, end);
+    chunk_of(a, part, begin, end);
     double2* scratch = smem;
     float* buf = reinterpret_cast<float*>(smem + kNormThreads / 32);
     float* counts = buf + 2 * (VEC / a.m) * sum_rows(a) * a.P;
@@ -716,8 +716,8 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
         block_moments<VEC>(v, pivot, in.n, a, pl, buf, counts);
     }
     __syncthreads();
-    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + blockIdx.x;
-    const double inv_n = (int)blockIdx.x < a.sums.more ? a.inv_long : a.inv_short;
+    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + part;
+    const double inv_n = part < a.sums.more ? a.inv_long : a.inv_short;
     group_sums<VEC>(a, buf, counts, scratch, [&](int g, double2 sums) {
         // the chunk's mean and sum of squares about it: 32 bits hold these
         const double mean = sums.x * inv_n;
@@ -924,9 +924,9 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
 {
     extern __shared__ double2 smem[];
     let_next_start();
-    const int b = a.image0 + blockIdx.y;
+    const int b = a.image0 + blockIdx.y, part = a.part0 + blockIdx.x * a.part_step;
     int begin, end;
-    chunk_of(a, blockIdx.x, begin, end);
+    chunk_of(a, part, begin, end);
     float2* stat = reinterpret_cast<float2*>(smem);
     float* params = reinterpret_cast<float*>(stat + a.G);
     float* chan = params + 2 * a.C;
@@ -954,11 +954,10 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         block_sums<VEC>(v, a, pl, buf);
     }
     __syncthreads();
-    const size_t part = (size_t)b * a.sums.count + blockIdx.x;
-    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + blockIdx.x;
+    float2* out = a.group_part + (size_t)b * a.sums.count * a.G + part;
     channel_and_group_sums<VEC>(a, params, buf, chan, [&](int g, double2 sums) { out[(size_t)g * a.sums.count] = make_float2((float)sums.x, (float)sums.y); });
     if (a.channel_part)
-        for (int c = threadIdx.x; c < a.C; c += blockDim.x) a.channel_part[part * a.C + c] = make_float2(chan[c], chan[a.C + c]);
+        for (int c = threadIdx.x; c < a.C; c += blockDim.x) a.channel_part[((size_t)b * a.sums.count + part) * a.C + c] = make_float2(chan[c], chan[a.C + c]);
     wait_previous();
 }
 

@@ -47,6 +47,7 @@ struct NormArgs
     int image0;       // first image of the launch
     NormParts sums;   // parts of an image that have a partial sum each
     NormParts own;    // parts that the blocks of the launch take
+    int part0, part_step;  // the sums' block k takes part part0 + k part_step
     double inv_n, inv_short, inv_long;     // 1 / values of a group in the image, in a part, in one with a row more
     int gather;           // log2 of the threads that add up a group's partial sums
     float inv_P, inv_Cg;

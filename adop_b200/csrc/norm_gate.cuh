@@ -157,7 +157,7 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v)
 
 // ---- activations --------------------------------------------------------------------------------------------------------
 constexpr float kLog2e = 1.4426950408889634f;
-// powers of two and reciprocals of the special-function unit (2 ulp; results below the smallest normal number become 0)
+// powers of two and reciprocals of the special-function unit (2 and 1 ulp; results below the smallest normal number become 0)
 __device__ __forceinline__ float ex2(float v)
 {
     float r;
@@ -173,7 +173,9 @@ __device__ __forceinline__ float rcp(float v)
 __device__ __forceinline__ float2 exp2v(float2 v) { return make_float2(ex2(v.x), ex2(v.y)); }
 __device__ __forceinline__ float2 rcp2(float2 v) { return make_float2(rcp(v.x), rcp(v.y)); }
 __device__ __forceinline__ float2 sigmoid(float2 v) { return rcp2(add(exp2v(mul(v, pair(-kLog2e))), pair(1.f))); }
-// sigmoid s and 1 - s = exp(-v) s, both to a few units of the last place. The exponential stays finite; where it would not, s is 0.
+// sigmoid s and 1 - s = exp(-v) s. The exponential's argument v log2(e) is rounded to 32 bits, which its result feels as 0.62 |v| ulp: s is within
+// (0.62 |v| + 4) 2^-23 of itself, 1 - s within (0.62 |v| + 7) 2^-23 (54 and 57 units at v = -80, where s is 2^-115; a
+// 16-bit result is rounded by up to 2^-11 of itself). Sigmoids below 2^-126, v < -87.3, are 0. The exponential stays finite; where it would not, s is 0.
 __device__ __forceinline__ float min_or_nan(float v, float most)
 {
     float r;

@@ -65,7 +65,9 @@ struct NormArgs
 };
 
 // Threads of a block and resident blocks of an SM that the kernels are compiled for: 64 registers forward and 80 backward, where a vector's
-// eight channels have four coefficients each. 256 threads with 128 registers hold too few vectors back from memory, 512 with 64 spill.
+// eight channels have four coefficients each. 256 threads with 128 registers hold too few vectors back from memory. Forward nothing spills;
+// backward some kernels of 16-byte vectors of 16-bit images spill 4 to 20 bytes (the last launch, gated or with SiLU, and the sums behind an
+// activation without a gate), with 512 threads and 64 registers all of them, 20 to 120 bytes.
 constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
 constexpr int kNormGradThreads = 384, kNormGradBlocks = 2;  // backward
 // vectors that the streaming kernels have under way for each thread: a power of two

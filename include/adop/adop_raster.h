@@ -482,7 +482,7 @@ adop_status adop_tonemap_backward(const adop_tonemap_params* p, const float* x, 
  *                          group, rstd = 1 / sqrt(var + eps), var without Bessel's correction
  *   adop_gated_activation  y = act(x) sigmoid(gate)
  * Images are channels-last with any pixel and image stride (a channel range of a wider image is one). Statistics and sums are
- * kept in 32 bits or more and every output is rounded once. Same inputs, same bits. */
+ * kept in 32 bits or more and every output is rounded once. Same inputs in the same layout, same bits. */
 #define ADOP_TYPE_F32 0
 #define ADOP_TYPE_F16 1
 #define ADOP_TYPE_BF16 2

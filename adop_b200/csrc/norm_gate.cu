@@ -147,16 +147,16 @@ Share share_of(const adop_norm_params* p, bool gated, bool backward)
     return {(int)images, (int)(chunks < 1 ? 1 : chunks)};
 }
 
-// A thread adds up kChain vectors at most in 32 bits before its sums go on in 64: n terms of one sign are off by n 2^-25 of their sum at worst, as
-// each addition rounds by 2^-24 of what there is by then. Where a block's share of an image is longer (2 MB of 16-byte vectors),
-// the sums take several launches, each over the next piece of every share. Two values in turn, the worst of their kind (the same term rounds the
-// same way), came out off by 2e-4 in float32 for 14000 vectors in one chain, by 2e-6 so. The launches cost nothing where they overlap (a 4K image of
-// 64 channels in bfloat16: 553 us forward with four as with one, 903 backward with five for 963) and 1 to 2 % where they cannot.
-constexpr int kChain = 256;
-int sum_launches(int64_t rows, int R, int chunks)
+// A thread adds up kChain vectors at most in 32 bits before its sums go on in 64, or in a second chain: n terms of one sign are off by n 2^-25 of
+// their sum at worst, as each addition rounds by 2^-24 of what there is by then. Where a block's share of an image is longer (2 MB of 16-byte
+// vectors; no image in memory where there is a second chain of as many), the sums take several launches, each over the next piece of every share.
+// Two values in turn, the worst of their kind (the same term rounds the same way), came out off by 2e-4 in float32 for 14000 vectors in one
+// chain, by 3e-6 so. The launches cost nothing where they overlap (a 4K image of 64 channels in bfloat16: 553 us forward with four as with one, 903
+// backward with five for 963) and 1 to 2 % where they cannot; second chains of wide vectors would spill, 2 % for all sizes backward.
+int sum_launches(int64_t rows, int V, int R, int chunks)
 {
-    const int64_t share = (rows + chunks - 1) / chunks;
-    return (int)((share + (int64_t)R * kChain - 1) / ((int64_t)R * kChain));
+    const int64_t share = (rows + chunks - 1) / chunks, most = (int64_t)R * kChain * (second_chain(V) ? kChain : 1);
+    return (int)((share + most - 1) / most);
 }
 // of the vectors that the tensors may turn out to allow, the ones that take most
 int most_sum_launches(const adop_norm_params* p, int chunks, bool backward)
@@ -167,7 +167,7 @@ int most_sum_launches(const adop_norm_params* p, int chunks, bool backward)
         const int common = (int)gcd64(p->channels, V);
         int R, threads;
         threads_of(p->channels / common, backward ? kNormGradThreads : kNormThreads, &R, &threads);
-        const int launches = sum_launches(p->pixels / (V / common), R, chunks);
+        const int launches = sum_launches(p->pixels / (V / common), V, R, chunks);
         if (launches > most) most = launches;
     }
     return most;
@@ -387,7 +387,7 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
     threads_of(a.P, kNormThreads, &a.R, &threads);
     const Share share = share_of(p, gated, false);
     const NormParts shares = parts_of(a.rows, share.chunks);
-    a.part_step = sum_launches(a.rows, a.R, shares.count);
+    a.part_step = sum_launches(a.rows, sh.V, a.R, shares.count);
     finish(&a, threads, (int64_t)shares.count * a.part_step);
     const size_t smem_stats = kWarpScratch + moments_scratch(sh, a.m, a.R, threads);
     const size_t smem_apply = apply_smem(a);
@@ -398,8 +398,8 @@ extern "C" adop_status adop_group_norm_forward(const adop_norm_params* p, const 
         a.vectors = (int)align16(smem_stats);
         a.own = a.sums;
         // Behind a gate a block has its SM busy: blocks that start early on SMs which the launch in front leaves free gather there, and the results'
-        // blocks after them (32 images of 960 x 540 x 16 in 128 blocks: 715 us, 505 us one launch after the other). With a block on every SM
-        // they find one place each (1920 x 1080 x 15: 187 us, 217 us).
+        // blocks after them (32 images of 960 x 540 x 16 in bfloat16, 128 blocks: 721 us, 503 us one launch after the other). With a block on every SM
+        // they find one place each (a 4K image of 32 channels in float32: 826 us, 857 us one after the other).
         const bool early = !gated || (int64_t)shares.count * n >= sm_count();
         for (a.part0 = 0; a.part0 < a.part_step; ++a.part0)
             ADOP_TRY(launch({"k_norm_stats", kNormStats, threads, dim3((unsigned)shares.count, n), stream_smem(smem_stats, sh, es, threads, gated, false),
@@ -462,7 +462,7 @@ extern "C" adop_status adop_group_norm_backward(const adop_norm_params* p, const
     ADOP_TRY(check_workspace(p, io, gated, true));
     const Share share = share_of(p, gated, true);
     const NormParts shares = parts_of(a.rows, share.chunks);
-    a.part_step = sum_launches(a.rows, a.R, shares.count);
+    a.part_step = sum_launches(a.rows, sh.V, a.R, shares.count);
     finish(&a, threads, (int64_t)shares.count * a.part_step);
     a.group_part = static_cast<float2*>(io->workspace);
     a.channel_part = params ? reinterpret_cast<float2*>(static_cast<char*>(io->workspace) + group_part_bytes(p, a.sums.count)) : nullptr;

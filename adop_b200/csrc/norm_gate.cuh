@@ -396,6 +396,11 @@ template <typename T, int VEC, bool GATED, bool GRAD> struct Stream
     }
     template <class Use> __device__ __forceinline__ void run(Use use)
     {
+        run_in<0>(use, [] {});
+    }
+    // fold() after every CHAIN vectors, a power of two
+    template <int CHAIN, class Use, class Fold> __device__ __forceinline__ void run_in(Use use, Fold fold)
+    {
         if constexpr (VEC > 1)
         {
             int i = 0;
@@ -407,6 +412,8 @@ template <typename T, int VEC, bool GATED, bool GRAD> struct Stream
                 use(a);
                 use(b);
                 copy(i + D, s);
+                if constexpr (CHAIN > 0)
+                    if (((i + 2) & (CHAIN - 1)) == 0) fold();
             }
             if (i < n)
             {
@@ -432,8 +439,29 @@ template <typename T, int VEC, bool GATED, bool GRAD> struct Stream
                 for (int k = 0; k < U; ++k)
                     if (i + k < n) use(in[k]);
                 x.on(U); g.on(U); d.on(U);
+                if constexpr (CHAIN > 0)
+                    if (((i + U) & (CHAIN - 1)) == 0) fold();
             }
         }
+    }
+    // the same where use() adds to v, two sums of each of a vector's lanes
+    template <class Use> __device__ __forceinline__ void sum(Lanes<VEC> (&v)[2], Use use)
+    {
+        if constexpr (second_chain(VEC))
+        {
+            Lanes<VEC> all[2];
+            all[0].fill(0.f); all[1].fill(0.f);
+            const auto join = [](Lanes<VEC>& to, const Lanes<VEC>& from) {
+#pragma unroll
+                for (int k = 0; k < Lanes<VEC>::N; ++k) to.p[k] = add(to.p[k], from.p[k]);
+            };
+            run_in<kChain>(use, [&] {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) { join(all[k], v[k]); v[k].fill(0.f); }
+            });
+            join(v[0], all[0]); join(v[1], all[1]);
+        }
+        else run(use);
     }
 };
 // u of a vector
@@ -710,7 +738,7 @@ __global__ void __launch_bounds__(kNormThreads, kNormBlocks) k_norm_stats(const 
         Stream<T, VEC, GATED, false> in(a, b, pl, begin, end, false, smem);
         in.start();
         bool have = false;
-        in.run([&](const Input<T, VEC>& i) {
+        in.sum(v, [&](const Input<T, VEC>& i) {
             const Lanes<VEC> u = value_of<T, VEC, GATED, ACT>(i, a.act);
             if (!have) pivot = pivot_of<VEC>(u, a.m);
             have = true;
@@ -952,7 +980,7 @@ __global__ void __launch_bounds__(kNormGradThreads, kNormGradBlocks) k_norm_grad
         {
             Saved<VEC> s;
             s.set(a, pl.ph, stat, params);
-            in.run([&](const Input<T, VEC>& i) { add_grad_sums<T, VEC, GATED, ACT>(i, s, v, a.act); });
+            in.sum(v, [&](const Input<T, VEC>& i) { add_grad_sums<T, VEC, GATED, ACT>(i, s, v, a.act); });
         }
         block_sums<VEC>(v, a, pl, buf);
     }

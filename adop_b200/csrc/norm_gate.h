@@ -72,6 +72,9 @@ constexpr int kNormThreads = 512, kNormBlocks = 2;          // forward
 constexpr int kNormGradThreads = 384, kNormGradBlocks = 2;  // backward
 // vectors that the streaming kernels have under way for each thread: a power of two
 __host__ __device__ constexpr int stream_depth(bool gated, bool grad) { return gated ? 4 : 8; }
+// vectors in a row that a thread adds up in 32 bits; those of one or two elements go on in a second chain then, which takes four registers
+constexpr int kChain = 256;
+__host__ __device__ constexpr bool second_chain(int vec) { return vec <= 2; }
 constexpr int kParamChannels = 32;  // channels whose parameters' gradients one block adds up
 
 const void* norm_kernel_f32(int which, int vec, bool gated, int act);

@@ -9,6 +9,7 @@ sums of one sign: e, and what uhat is off by."""
 import pytest
 import torch
 
+from adop_b200 import capi
 from tests.test_norm_gate_gpu import DEV, Reference, call, check, eight_sm_stream, image, op  # noqa: F401 (two are fixtures)
 
 pytestmark = pytest.mark.gpu
@@ -53,12 +54,15 @@ def test_two_values_in_turn(op, dtype, channels, pixels, offset):
         assert (dx[:, :, 0, k::2].double() - want).abs().max().item() <= bound
 
 
-def long_case(kind, seed):
-    """A 1080p image whose address allows single elements only: two launches of sums and more, forward and backward."""
+def long_case(kind, size, seed):
+    """Channels 4 to 19 (35) of wider images: vectors of 8 bytes, 438 of them for a thread of a 4K image, 512 for one of each of 75 blocks (which, behind a gate,
+    do not overlap), a third more backward."""
     gen = torch.Generator(device=DEV).manual_seed(seed)
-    x = image((1, 16 if kind == "norm" else 32, 1080, 1920), torch.bfloat16, gen, "odd_slice").requires_grad_(True)
+    B, H, W = size
+    C = 16 if kind == "norm" else 32
+    x = image((B, C + 4, H, W), torch.bfloat16, gen)[:, 4:].detach().requires_grad_(True)
     w, b = (torch.randn(16, device=DEV, generator=gen).requires_grad_(True) for _ in range(2))
-    return x, w, b, image((1, 16, 1080, 1920), torch.bfloat16, gen)
+    return x, w, b, image((B, 16, H, W), torch.bfloat16, gen)
 
 
 def step(op, kind, x, w, b, dy):
@@ -66,10 +70,22 @@ def step(op, kind, x, w, b, dy):
     return [y.detach(), *torch.autograd.grad(y, [x, w, b], dy)]
 
 
+def test_several_launches_are_what_these_are(op, cuda_lib):
+    for kind, size in (("norm", (1, 2160, 3840)), ("gated_norm", (75, 256, 256))):
+        x, w, b, _ = long_case(kind, size, 0)
+        capi.profile_enable(True)
+        call(op, kind, x, 4, w, b, 1e-5, "silu")
+        torch.cuda.synchronize()
+        times = capi.profile_collect()
+        capi.profile_enable(False)
+        assert times["k_norm_stats"][0] > times["k_norm_apply"][0]
+
+
+@pytest.mark.parametrize("size", [(1, 2160, 3840), (75, 256, 256)], ids=str)
 @pytest.mark.parametrize("kind", ["norm", "gated_norm"])
-def test_several_launches_of_sums(op, kind, eight_sm_stream):
+def test_several_launches_of_sums(op, kind, size, eight_sm_stream):
     """The values; and the same bits again, on two streams at once, on a stream with a part of the GPU and from a graph."""
-    cases = [long_case(kind, k) for k in range(2)]
+    cases = [long_case(kind, size, k) for k in range(2)]
     want = [step(op, kind, *c) for c in cases]
     x, w, b, dy = cases[0]
     ref = Reference(kind, x, 4, w, b, 1e-5, "silu", dy)

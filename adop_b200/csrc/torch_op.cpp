@@ -523,7 +523,8 @@ static Tensor as_stored(const Tensor& t) { return t.defined() && t.is_neg() ? t.
 static Tensor channels_last(const Tensor& t)
 {
     int64_t stride;
-    return as_stored(t.numel() == 0 || pixel_stride(t, &stride) ? t : t.contiguous(torch::MemoryFormat::ChannelsLast));
+    if (t.numel() == 0 || pixel_stride(t, &stride)) return as_stored(t);
+    return as_stored(t.contiguous(torch::MemoryFormat::ChannelsLast));
 }
 // channels [c0, ...) of t
 static adop_norm_image norm_image(const Tensor& t, int64_t c0 = 0)

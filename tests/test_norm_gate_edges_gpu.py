@@ -7,6 +7,7 @@ unit more, (0.62 |v| + 4) 2^-23 of s; 1 - s = exp(-v) s another exponential's tw
 exponential's argument enters both, at most once in all. Sigmoids below 2^-126 are 0. Where a feature's activation and its slope come with
 exponentials of their own, 2^-18 as in the other tests."""
 import ctypes as C
+import gc
 
 import pytest
 import torch
@@ -15,6 +16,14 @@ from adop_b200 import capi
 from tests.test_norm_gate_gpu import ACTS, DEV, TYPES, Reference, act64, call, check, half_step, image, op, run_case, slope64  # noqa: F401 (op is a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def gigabytes_given_back():
+    """What later tests keep is not to lie in a cached block of these ones' sizes."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 ULP = 2.0 ** -23
 

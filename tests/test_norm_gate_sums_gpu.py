@@ -6,6 +6,8 @@ sum so far at most, half the last on average, so e = 2^-17 of the sum. With d = 
 squares about the mean, sum(d)^2 / n as much as these, so the squares about the mean are off by 2 e + 2 e of themselves, the variance by 4 e and
 rstd by 2 e; the mean by e D / 2, which is e of the spread. uhat = +-1 is off by 3 e, and by 2^-22 |mean| rstd as everywhere. db and dw are
 sums of one sign: e, and what uhat is off by."""
+import gc
+
 import pytest
 import torch
 
@@ -13,6 +15,14 @@ from adop_b200 import capi
 from tests.test_norm_gate_gpu import DEV, Reference, call, check, eight_sm_stream, image, op  # noqa: F401 (two are fixtures)
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, scope="module")
+def gigabytes_given_back():
+    """What later tests keep is not to lie in a cached block of these ones' sizes."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
 
 E = 2.0 ** -17
 
